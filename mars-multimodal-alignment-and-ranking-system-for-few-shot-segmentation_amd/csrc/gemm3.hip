@@ -562,8 +562,7 @@ __global__ __launch_bounds__(64 * NWR * NWC, WPE) void gemm_tn_ring_kernel(MarsG
                     else x[e] = g.alpha * a0 + bias_[v][e];
                 }
                 if constexpr (MODE == 1 && FAST) {
-                    // QuickGELU two outputs at a time: the multiplies and the add around the two transcendentals
-                    // are packed instructions (act_fn3 per element leaves them single)
+                    // QuickGELU two outputs at a time, one's transcendentals under the other's arithmetic
 #pragma unroll
                     for (int e = 0; e < VW; e += 2) {
                         const f32x2 y = {x[e], x[e + 1]};

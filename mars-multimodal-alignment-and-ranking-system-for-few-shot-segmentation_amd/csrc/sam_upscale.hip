@@ -34,8 +34,8 @@ __device__ __forceinline__ float halves_sum(float a) { return halves_sum2(a, a);
 
 // 0.5 v (1 + erf(v / sqrt 2)), erf by Abramowitz & Stegun 7.1.26 (absolute error below 1.5e-7, i.e. f32 rounding
 // level for the activations here): erf(z) = 1 - (a1 t + ... + a5 t^5) exp(-z^2), t = 1 / (1 + p z), z >= 0; the result
-// is v - v e / 2 for v >= 0 and -|v| e / 2 below.  Two values at a time: the multiplies and multiply-adds are
-// v_pk_*_f32 (two values an issue slot); only the reciprocal and the exponential stay one value an instruction.
+// is v - v e / 2 for v >= 0 and -|v| e / 2 below.  Two values at a time, so that one's reciprocal and exponential
+// are in flight under the other's multiply-adds (the build makes no packed f32 instructions of the pairs).
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ f32x2 gelu_erf2(f32x2 v) {
     const f32x2 a = __builtin_elementwise_abs(v), z = a * 0.70710678118654752440f;

@@ -12,18 +12,12 @@ __global__ __launch_bounds__(512) void rate_kernel(float* out, unsigned long lon
     float a[8];
     for (int i = 0; i < 8; ++i) a[i] = -0.001f * (threadIdx.x + i);
     float b0 = 1.0001f, b1 = 0.5f;
-    typedef float f2 __attribute__((ext_vector_type(2)));
-    f2 p[4] = {{a[0], a[1]}, {a[2], a[3]}, {a[4], a[5]}, {a[6], a[7]}};
-    f2 q = {b0, b1};
     const unsigned long long t0 = __builtin_amdgcn_s_memtime();
     for (int it = 0; it < iters; ++it) {
         if (WHICH == 0) { REP8(asm volatile("v_exp_f32 %0, %0\n v_exp_f32 %1, %1\n v_exp_f32 %2, %2\n v_exp_f32 %3, %3" : "+v"(a[0]), "+v"(a[1]), "+v"(a[2]), "+v"(a[3]));) }
         if (WHICH == 1) { REP8(asm volatile("v_mul_f32 %0, %0, %4\n v_mul_f32 %1, %1, %4\n v_mul_f32 %2, %2, %4\n v_mul_f32 %3, %3, %4" : "+v"(a[0]), "+v"(a[1]), "+v"(a[2]), "+v"(a[3]) : "v"(b0));) }
-        if (WHICH == 2) { REP8(asm volatile("v_pk_mul_f32 %0, %0, %4\n v_pk_mul_f32 %1, %1, %4\n v_pk_mul_f32 %2, %2, %4\n v_pk_mul_f32 %3, %3, %4" : "+v"(p[0]), "+v"(p[1]), "+v"(p[2]), "+v"(p[3]) : "v"(q));) }
         if (WHICH == 3) { REP8(asm volatile("v_exp_f16 %0, %0\n v_exp_f16 %1, %1\n v_exp_f16 %2, %2\n v_exp_f16 %3, %3" : "+v"(a[0]), "+v"(a[1]), "+v"(a[2]), "+v"(a[3]));) }
         if (WHICH == 4) { REP8(asm volatile("v_cvt_pk_bf16_f32 %0, %0, %1\n v_cvt_pk_bf16_f32 %1, %1, %2\n v_cvt_pk_bf16_f32 %2, %2, %3\n v_cvt_pk_bf16_f32 %3, %3, %0" : "+v"(a[0]), "+v"(a[1]), "+v"(a[2]), "+v"(a[3]));) }
-        if (WHICH == 5) { REP8(asm volatile("v_exp_f32 %0, %0\n v_pk_mul_f32 %4, %4, %6\n v_exp_f32 %1, %1\n v_pk_mul_f32 %5, %5, %6\n v_exp_f32 %2, %2\n v_pk_mul_f32 %4, %4, %6\n v_exp_f32 %3, %3\n v_pk_mul_f32 %5, %5, %6" : "+v"(a[0]), "+v"(a[1]), "+v"(a[2]), "+v"(a[3]), "+v"(p[0]), "+v"(p[1]) : "v"(q));) }
-        if (WHICH == 6) { REP8(asm volatile("v_pk_fma_f32 %0, %0, %4, %4\n v_pk_fma_f32 %1, %1, %4, %4\n v_pk_fma_f32 %2, %2, %4, %4\n v_pk_fma_f32 %3, %3, %4, %4" : "+v"(p[0]), "+v"(p[1]), "+v"(p[2]), "+v"(p[3]) : "v"(q));) }
         if (WHICH == 7) { REP8(asm volatile("v_add_f32 %0, %0, %4\n v_add_f32 %1, %1, %4\n v_add_f32 %2, %2, %4\n v_add_f32 %3, %3, %4" : "+v"(a[0]), "+v"(a[1]), "+v"(a[2]), "+v"(a[3]) : "v"(b1));) }
         if (WHICH == 8) { REP8(asm volatile("v_ldexp_f32 %0, %0, %4\n v_ldexp_f32 %1, %1, %4\n v_ldexp_f32 %2, %2, %4\n v_ldexp_f32 %3, %3, %4" : "+v"(a[0]), "+v"(a[1]), "+v"(a[2]), "+v"(a[3]) : "v"(1));) }
         if (WHICH == 10) { REP32(asm volatile("v_mul_f32 %0, %0, %1" : "+v"(a[0]) : "v"(b0));) }
@@ -35,7 +29,6 @@ __global__ __launch_bounds__(512) void rate_kernel(float* out, unsigned long lon
     const unsigned long long t1 = __builtin_amdgcn_s_memtime();
     float s = 0;
     for (int i = 0; i < 8; ++i) s += a[i];
-    for (int i = 0; i < 4; ++i) s += p[i][0] + p[i][1];
     out[blockIdx.x * blockDim.x + threadIdx.x] = s;
     if ((threadIdx.x & 63) == 0) cyc[blockIdx.x * (blockDim.x / 64) + threadIdx.x / 64] = t1 - t0;
 }
@@ -65,11 +58,8 @@ int main() {
     run<7>("v_add_f32", 32, out, cyc);
     run<0>("v_exp_f32", 32, out, cyc);
     run<3>("v_exp_f16", 32, out, cyc);
-    run<2>("v_pk_mul_f32", 32, out, cyc);
-    run<6>("v_pk_fma_f32", 32, out, cyc);
     run<4>("v_cvt_pk_bf16_f32", 32, out, cyc);
     run<8>("v_ldexp_f32", 32, out, cyc);
     run<9>("v_max3_f32", 32, out, cyc);
-    run<5>("exp + pk_mul pairs", 64, out, cyc);
     return 0;
 }
