@@ -168,6 +168,72 @@ int marship_flash_attn_fp8(const void* qkv, void* O, int B, int T, int H, void* 
 int marship_flash_attn_mean(const void* qkv, const float* lse, int T, int H, int off, int Pn,
                             float scale, float* acc, int64_t ldacc, float score_scale_log2, void* stream);
 
+/* ---- attention between two token sets --------------------------------------------- */
+/* softmax(scale q.k + bias) v of Lq query tokens over the attended ones of Lk key tokens (no counterpart in the reference, whose
+ * one attention between two sets is the mask decoder's: marship_attn_small).  Everything is a strided view, strides in
+ * elements in the order (batch entry, token, head), the elements of a head contiguous, rows 16-byte aligned; hd <= 128,
+ * hd elements a multiple of 16 bytes.  dtype (0 f32, 1 bf16) is that of q, k, v, out and their gradients; products, scores, statistics and
+ * sums are f32 (f32 operands go through the f32 matrix instructions).
+ *   H query heads share Hkv key heads in order: query head h reads key head h / (H / Hkv).
+ *   kv_len i32 [B] (may be NULL): keys at or behind it are not attended (clamped to 0 .. Lk).  mask u8 [B, Lk], contiguous (may be NULL): keys
+ *   with 0 are not attended.  What K and V hold at keys that are not attended is not read.
+ *   bias f32 [H, Lq, Lk] by bias_s = (head, query row), shared by the batch (may be NULL); -inf and the lowest float are allowed.
+ * A row without a key (none attended, or a bias of -inf on all of them) gives zeros and stat (-inf, 0).
+ * stat f32 [B, H, Lq, 2]: maximum of the row's scores and sum of exp(score - maximum); written by the forward call where not NULL, read by the
+ * backward one.
+ * Backward: dq, dk, dv (dk, dv: zeros at keys not attended) and, where dbias is not NULL, dbias f32 [H, Lq, Lk] by dbias_s, summed over the
+ * batch.  Sums have a fixed order: results do not change from call to call.
+ * ws: workspace of at least marship_cross_attn_ws(args, backward) bytes, 16-byte aligned, of the caller's and not shared
+ * with a call that may run at the same time (it may be NULL where that is 0). */
+typedef struct {
+    const void *q, *k, *v;
+    void* out;
+    float* stat;
+    const float* bias;
+    const int32_t* kv_len;
+    const uint8_t* mask;
+    int64_t q_s[3], k_s[3], v_s[3], out_s[3], bias_s[2];
+    int32_t B, Lq, Lk, H, Hkv, hd;
+    float scale;
+    int32_t dtype;
+    const void* dout;
+    void *dq, *dk, *dv;
+    float* dbias;
+    int64_t dout_s[3], dq_s[3], dk_s[3], dv_s[3], dbias_s[2];
+    void* ws;
+    int64_t ws_bytes;
+} MarsCrossAttn;
+int64_t marship_cross_attn_ws(const MarsCrossAttn* args, int backward);
+int marship_cross_attn(const MarsCrossAttn* args, void* stream);
+int marship_cross_attn_bwd(const MarsCrossAttn* args, void* stream);
+
+/* ---- learned relative-position bias by buckets -------------------------------------- */
+/* bias[h, (qy, qx), (ky, kx)] = table[by[ky - qy + qh - 1], bx[kx - qx + qw - 1], h] for query tokens on a qh x qw grid and key tokens on a
+ * kh x kw grid (a line of tokens: one row, by = {0}).  No counterpart in the reference (its one position bias is the decomposed,
+ * query-dependent one of image_encoder.py:325-361: marship_relpos_bias).  table f32 [ny, nx, H]; by i32 [qh + kh - 1], bx i32 [qw + kw - 1]
+ * (an entry outside 0 .. ny - 1 / 0 .. nx - 1: no bias and no gradient at those offsets); bias and dbias f32 [H, qh qw, kh kw] with strides s_head, s_row
+ * in elements.  Backward: dtable f32 [ny, nx, H], every entry written, sums in a fixed order; ws: at least
+ * marship_bucket_bias_bwd_ws bytes, 16-byte aligned. */
+int marship_bucket_bias(const float* table, const int32_t* by, const int32_t* bx, float* out, int64_t s_head, int64_t s_row, int H, int qh, int qw,
+                        int kh, int kw, int ny, int nx, void* stream);
+int64_t marship_bucket_bias_bwd_ws(int H, int qh, int qw, int kh, int kw, int nx);
+int marship_bucket_bias_bwd(const float* dbias, int64_t s_head, int64_t s_row, const int32_t* by, const int32_t* bx, float* dtable, int H, int qh,
+                            int qw, int kh, int kw, int ny, int nx, void* ws, int64_t ws_bytes, void* stream);
+
+/* ---- group norm with an activation, channels last ------------------------------------ */
+/* x [N, P, C] (strides x_n, x_p in elements, channels contiguous), G groups of C / G neighbouring channels:
+ * out = act(w (x - mean) rstd + b) with the mean and variance of a group's P C / G values.  No counterpart in the reference (its channels-last
+ * norm is LayerNorm2d: marship_layernorm_act_rows).  act: 0 none, 1 erf GELU, 2 QuickGELU, 3 ReLU, 4 SiLU.  x and out f32 or bf16 each; w, b f32 [C].
+ * stat f32 [N, G, 2] receives mean and rstd where not NULL; the backward call reads it.
+ * Backward: dx (x's dtype), dw, db f32 [C]; dy f32 or bf16.  Statistics and sums are f32 in a fixed order.  ws: at least
+ * marship_group_norm_act_ws bytes, 16-byte aligned. */
+int64_t marship_group_norm_act_ws(int N, int P, int C, int G, int backward);
+int marship_group_norm_act(const void* x, int64_t x_n, int64_t x_p, const float* w, const float* b, void* out, int64_t o_n, int64_t o_p, int N, int P,
+                           int C, int G, float eps, int act, int x_dtype, int out_dtype, float* stat, void* ws, int64_t ws_bytes, void* stream);
+int marship_group_norm_act_bwd(const void* x, int64_t x_n, int64_t x_p, const float* w, const float* b, const float* stat, const void* dy, int64_t dy_n,
+                               int64_t dy_p, void* dx, int64_t dx_n, int64_t dx_p, float* dw, float* db, int N, int P, int C, int G, int act,
+                               int x_dtype, int dy_dtype, void* ws, int64_t ws_bytes, void* stream);
+
 /* ---- alignment / refinement ------------------------------------------------------ */
 /* F.normalize(p=2, dim=1) on gathered rows (VisualVisualAlignmentModule.py:122-125;
  * FilteringMergingModule.py:179,200).  Row r of image b is x + b*x_bstride + (row_off+r)*x_stride. */

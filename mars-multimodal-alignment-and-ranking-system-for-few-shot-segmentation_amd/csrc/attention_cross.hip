@@ -1,0 +1,469 @@
+// Attention of one set of tokens over another of another length (query patches over support patches; prompt tokens over
+// an image; a new token over an encoder's states), forward:
+//
+//   s_ij = scale q_i . k_j + bias[h, i, j] over the attended keys,   o_i = sum_j softmax_j(s_ij) v_j
+//
+// One pass over the keys with a running maximum and sum.  A wave owns 32 query rows and computes S^T = K Q^T on the
+// 32x32 matrix instructions, so that a query is a lane column: row statistics are per-lane values that meet in one
+// half-wave swap, and the exponentials are, as they stand, the operand of O^T += V^T P^T.
+//
+// Masked keys are not computed and then thrown away: where the caller gives a mask, a first launch lists the attended keys of each
+// batch entry, and the fills gather K and V rows through that list.  A support image's foreground is a tenth to
+// a half of its patches, a row costs the same gathered or not (it is at least one 32-byte sector, mostly one or two cache lines),
+// and whatever stands in a masked row - infinities, NaN - is never read.
+#include "attention_cross.h"
+
+namespace xattn {
+namespace {
+
+// ------------------------------------------------------------------------------------------------ lists of attended keys
+// idx[b] = attended keys in order, then the others in order; cnt[b] = how many.  A workgroup of 1024 per batch entry: ballots
+// within a wave, a scan over its sixteen waves, 1024 keys a step.
+__global__ __launch_bounds__(1024) void list_keys_kernel(const uint8_t* __restrict__ mask, const int32_t* __restrict__ kv_len, int Lk,
+                                                         int32_t* __restrict__ idx, int32_t* __restrict__ cnt) {
+    __shared__ int wsum[16];
+    const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const uint8_t* m = mask + (int64_t)b * Lk;
+    const int len = kv_len == nullptr ? Lk : min(max(kv_len[b], 0), Lk);
+    int32_t* out = idx + (int64_t)b * Lk;
+    auto scan = [&](int total0, auto emit) {
+        int total = total0;
+        for (int j0 = 0; j0 < Lk; j0 += 1024) {
+            const int j = j0 + tid;
+            const bool on = j < len && m[j] != 0;
+            const unsigned long long bal = __ballot(on);
+            const int before = __popcll(bal & ((1ull << lane) - 1));
+            __syncthreads();
+            if (lane == 0) wsum[wave] = __popcll(bal);
+            __syncthreads();
+            int base = total;
+            for (int w = 0; w < wave; ++w) base += wsum[w];
+            for (int w = 0; w < 16; ++w) total += wsum[w];
+            if (j < Lk) emit(j, on, base + before);
+        }
+        return total;
+    };
+    const int n = scan(0, [&](int j, bool on, int pos) { if (on) out[pos] = j; });
+    // an unattended key stands behind the n attended ones, after the unattended keys before it
+    scan(0, [&](int j, bool on, int pos) { if (!on) out[n + j - pos] = j; });
+    if (tid == 0) cnt[b] = n;
+}
+
+// ------------------------------------------------------------------------------------------------ forward
+struct Fwd {
+    Prob p;
+    void* out;                      // [B, Lq, H, hd] by p.so, or nullptr where there are partial results to join
+    float* stat;                    // [B, H, Lq, 2]: row maximum and sum of exp(s - maximum); may be nullptr
+    float *part_o, *part_s;         // partial results: [ns][B Hkv][R][HDP] un-normalised, [ns][B Hkv][R][2]
+    int nrb, ns;                    // row blocks, splits of the keys
+};
+
+// FEW: at most 32 rows: the four waves share them and take key tiles in turn, each through LDS buffers of its own (no barrier),
+// and join their results at the end.  Otherwise each wave has 32 rows of a 128-row block and the workgroup shares the tiles.
+template <typename T, int HDP, bool FEW> struct FwdCfg {
+    static constexpr int KT = FEW ? 32 : 64;                                             // keys per tile
+    static constexpr int TB = KT * HDP * (int)sizeof(T);
+    static constexpr int COPIES = FEW ? 4 : 1;
+    static constexpr int BUFS = COPIES * 4 * TB <= 128 * 1024 ? 2 : 1;
+    static constexpr int WPE = COPIES * BUFS * 2 * TB <= 80 * 1024 ? 2 : 1;              // waves a SIMD that the LDS leaves room for
+};
+
+template <typename T, int HDP, bool BIAS, bool FEW>
+__global__ __launch_bounds__(256, (FwdCfg<T, HDP, FEW>::WPE)) void cross_fwd_kernel(const Fwd f) {
+    using Cfg = FwdCfg<T, HDP, FEW>;
+    using TL = Tile<T, HDP>;
+    constexpr int KT = Cfg::KT, TB = Cfg::TB, KB = KT / 32, KS = HDP / 16, DM = HDP / 32;
+    __shared__ __attribute__((aligned(16))) unsigned char buf0[Cfg::COPIES][2][TB];
+    __shared__ __attribute__((aligned(16))) unsigned char buf1[Cfg::BUFS == 2 ? Cfg::COPIES : 1][Cfg::BUFS == 2 ? 2 : 1][Cfg::BUFS == 2 ? TB : 16];
+    const Prob& p = f.p;
+    const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int cw = FEW ? wave : 0;                              // which copy of the buffers
+    int bh, blk;
+    place_block(blockIdx.x, p.B * p.Hkv, f.nrb * f.ns, bh, blk);
+    const int rb = blk % f.nrb, split = blk / f.nrb;
+    const int b = bh / p.Hkv, hk = bh - b * p.Hkv;
+    const int r = FEW ? rb * 32 + (lane & 31) : rb * 128 + wave * 32 + (lane & 31);
+    const bool row_ok = r < p.R;
+    int l = 0, h = 0;
+    if (row_ok) row_of(p, hk, r, l, h);
+    frag_t<T> qf[KS];
+    const T* qrow = row_ok ? row_ptr<T>(p.q, p.sq, b, l, h) : nullptr;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = load_frag<T>(qrow, ks, hh, p.hd);
+    const float* brow = BIAS && row_ok ? p.bias + h * p.bias_h + l * p.bias_l : nullptr;
+
+    const int n = key_count(p, b);
+    const int32_t* idx = p.idx == nullptr ? nullptr : p.idx + (int64_t)b * p.Lk;
+    int t0, t1;
+    split_range((n + KT - 1) / KT, split, f.ns, t0, t1);
+    const int hdb = p.hd * (int)sizeof(T);
+    const unsigned char* kbase = (const unsigned char*)row_ptr<T>(p.k, p.sk, b, 0, hk);
+    const unsigned char* vbase = (const unsigned char*)row_ptr<T>(p.v, p.sv, b, 0, hk);
+    const int64_t kl = p.sk.l * (int)sizeof(T), vl = p.sv.l * (int)sizeof(T);
+
+    auto issue = [&](int t, unsigned char* dst) {
+        constexpr int NW = FEW ? 1 : 4;
+        const int w = FEW ? 0 : wave;
+        // (keys behind the last attended one: that one again - their scores are set to -inf, and its row holds no value that the
+        // sums would not see anyway)
+        TL::template fill<KT, NW>(dst, w, lane, hdb, [&](int row) { return kbase + key_row(idx, min(t * KT + row, n - 1)) * kl; });
+        TL::template fill<KT, NW>(dst + TB, w, lane, hdb, [&](int row) { return vbase + key_row(idx, min(t * KT + row, n - 1)) * vl; });
+    };
+
+    f32x16 o[DM];
+#pragma unroll
+    for (int m = 0; m < DM; ++m) o[m] = zero16();
+    float mrun = -INFINITY, lsum = 0.f;
+    const float c2 = p.scale * LOG2E;
+
+    // one tile: scores, running maximum, exponentials, products with V.  Without a bias the maximum is of the raw products
+    // (scale > 0) and scale and log2 e come with the exponent; with one the scores are kept in natural units, because
+    // a mask made of the type's lowest value would overflow in units of log 2.
+    auto tile = [&](int t, const unsigned char* kt, const unsigned char* vt) {
+        f32x16 s[KB];
+        const bool ragged = t * KT + KT > n;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+            s[kb] = zero16();
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) s[kb] = mma(TL::rows(kt, 32 * kb, ks, lane), qf[ks], s[kb]);
+            if constexpr (BIAS) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int j = min(t * KT + 32 * kb + acc_row(i, hh), n - 1);
+                    s[kb][i] = fmaf(s[kb][i], p.scale, brow != nullptr ? brow[key_row(idx, j)] : 0.f);
+                }
+            }
+            if (ragged) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (t * KT + 32 * kb + acc_row(i, hh) >= n) s[kb][i] = -INFINITY;
+            }
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb][i]);
+        const float mnew = fmaxf(mrun, halves_max(mx));
+        // (a bias of -inf on every key so far: nothing to scale, and the exponentials must come out as zeros)
+        const float mref = BIAS && mnew == -INFINITY ? 0.f : mnew;
+        const float unit = BIAS ? LOG2E : c2;
+        const float alpha = __builtin_amdgcn_exp2f((mrun - mref) * unit);
+        mrun = mnew;
+        lsum *= alpha;
+        const float sub = mref * unit;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[kb][i] = __builtin_amdgcn_exp2f(BIAS ? (s[kb][i] - mref) * unit : fmaf(s[kb][i], unit, -sub));
+                lsum += s[kb][i];
+            }
+        if (!__all(alpha == 1.f)) {
+#pragma unroll
+            for (int m = 0; m < DM; ++m)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[m][i] *= alpha;
+        }
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                // probabilities of bf16 heads are rounded to bf16 for the matrix instruction (half a step, 2^-9 of each, with signs
+                // that do not agree: far below the rounding of the result); their sum is taken before the rounding
+                const frag_t<T> pf = pack_step<T>(s[kb], u);
+#pragma unroll
+                for (int m = 0; m < DM; ++m) o[m] = mma(TL::cols(vt, 32 * kb + 16 * u, m, lane), pf, o[m]);
+            }
+    };
+
+    if constexpr (!FEW) {
+        if (t0 < t1) issue(t0, buf0[0][0]);
+        if constexpr (Cfg::BUFS == 2) {
+            for (int t = t0; t < t1; t += 2) {
+                __syncthreads();
+                if (t + 1 < t1) issue(t + 1, buf1[0][0]);
+                tile(t, buf0[0][0], buf0[0][1]);
+                if (t + 1 < t1) {
+                    __syncthreads();
+                    if (t + 2 < t1) issue(t + 2, buf0[0][0]);
+                    tile(t + 1, buf1[0][0], buf1[0][1]);
+                }
+            }
+        } else {
+            for (int t = t0; t < t1; ++t) {
+                __syncthreads();
+                tile(t, buf0[0][0], buf0[0][1]);
+                __syncthreads();
+                if (t + 1 < t1) issue(t + 1, buf0[0][0]);
+            }
+        }
+    } else {
+        unsigned char* my0 = buf0[cw][0];
+        unsigned char* my1 = Cfg::BUFS == 2 ? buf1[Cfg::BUFS == 2 ? cw : 0][0] : my0;
+        // waves without a tile skip the loops; a wave's own buffers need its own waits only
+        const int first = t0 + wave;
+        if (first < t1) issue(first, my0);
+        if constexpr (Cfg::BUFS == 2) {
+            for (int t = first; t < t1; t += 8) {
+                __builtin_amdgcn_s_waitcnt(0);
+                if (t + 4 < t1) issue(t + 4, my1);
+                tile(t, my0, my0 + TB);
+                if (t + 4 < t1) {
+                    __builtin_amdgcn_s_waitcnt(0);
+                    if (t + 8 < t1) issue(t + 8, my0);
+                    tile(t + 4, my1, my1 + TB);
+                }
+            }
+        } else {
+            for (int t = first; t < t1; t += 4) {
+                __builtin_amdgcn_s_waitcnt(0);
+                tile(t, my0, my0 + TB);
+                __builtin_amdgcn_s_waitcnt(0);
+                if (t + 4 < t1) issue(t + 4, my0);
+            }
+        }
+    }
+    lsum = halves_sum(lsum);
+
+    if constexpr (FEW) {
+        // join the waves: maxima and sums, then the rescaled accumulators, wave by wave through LDS
+        float* xs = (float*)buf0[0][0];                         // [4][32][2]
+        float* xo = xs + 4 * 32 * 2;                            // [32][HDP + 4]
+        static_assert((4 * 32 * 2 + 32 * (HDP + 4)) * 4 <= Cfg::COPIES * 2 * TB, "the exchange fits the tile buffers");
+        __syncthreads();
+        if (hh == 0) { xs[(wave * 32 + lane) * 2] = mrun; xs[(wave * 32 + lane) * 2 + 1] = lsum; }
+        __syncthreads();
+        float mall = -INFINITY, lall = 0.f;
+        for (int w = 0; w < 4; ++w) mall = fmaxf(mall, xs[(w * 32 + (lane & 31)) * 2]);
+        const float mref = mall == -INFINITY ? 0.f : mall;
+        const float unit = BIAS ? LOG2E : c2;
+        for (int w = 0; w < 4; ++w) {
+            const float mw = xs[(w * 32 + (lane & 31)) * 2];
+            lall += xs[(w * 32 + (lane & 31)) * 2 + 1] * __builtin_amdgcn_exp2f((mw - mref) * unit);
+        }
+        const float mine = __builtin_amdgcn_exp2f((mrun - mref) * unit);
+        for (int w = 3; w >= 0; --w) {
+            if (wave == w) {
+#pragma unroll
+                for (int m = 0; m < DM; ++m)
+#pragma unroll
+                    for (int a = 0; a < 4; ++a) {
+                        float* x = xo + (lane & 31) * (HDP + 4) + 32 * m + 8 * a + 4 * hh;
+                        f32x4 v = {o[m][4 * a] * mine, o[m][4 * a + 1] * mine, o[m][4 * a + 2] * mine, o[m][4 * a + 3] * mine};
+                        if (w < 3) { const f32x4 c = *(const f32x4*)x; v[0] += c[0]; v[1] += c[1]; v[2] += c[2]; v[3] += c[3]; }
+                        if (w > 0) *(f32x4*)x = v;
+                        else { o[m][4 * a] = v[0]; o[m][4 * a + 1] = v[1]; o[m][4 * a + 2] = v[2]; o[m][4 * a + 3] = v[3]; }
+                    }
+            }
+            __syncthreads();
+        }
+        if (wave != 0) return;
+        mrun = mall;
+        lsum = lall;
+    }
+
+    if (!row_ok) return;
+    const float mnat = BIAS ? mrun : mrun * p.scale;
+    if (f.ns > 1) {
+        const int64_t row = ((int64_t)split * p.B * p.Hkv + bh) * p.R + r;
+        float* po = f.part_o + row * HDP;
+#pragma unroll
+        for (int m = 0; m < DM; ++m)
+#pragma unroll
+            for (int a = 0; a < 4; ++a) *(f32x4*)(po + 32 * m + 8 * a + 4 * hh) = (f32x4){o[m][4 * a], o[m][4 * a + 1], o[m][4 * a + 2], o[m][4 * a + 3]};
+        if (hh == 0) { f.part_s[row * 2] = mnat; f.part_s[row * 2 + 1] = lsum; }
+        return;
+    }
+    const float inv = lsum == 0.f ? 0.f : 1.0f / lsum;          // a row without keys: zeros
+    T* orow = (T*)f.out + b * p.so.b + l * p.so.l + h * p.so.h;
+#pragma unroll
+    for (int m = 0; m < DM; ++m)
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+            const int d = 32 * m + 8 * a + 4 * hh;
+            if (d < p.hd) store4(orow + d, o[m][4 * a] * inv, o[m][4 * a + 1] * inv, o[m][4 * a + 2] * inv, o[m][4 * a + 3] * inv);
+        }
+    if (f.stat != nullptr && hh == 0) {
+        float* st = f.stat + (((int64_t)b * p.H + h) * p.Lq + l) * 2;
+        st[0] = mnat;
+        st[1] = lsum;
+    }
+}
+
+// joins the splits: 64 / (HDP / 4) rows a wave, a lane owns four elements of a row
+template <typename T, int HDP>
+__global__ __launch_bounds__(256) void cross_join_kernel(const Fwd f) {
+    constexpr int LR = HDP / 4;
+    const Prob& p = f.p;
+    const int64_t rows = (int64_t)p.B * p.Hkv * p.R;
+    const int64_t g = (int64_t)blockIdx.x * (256 / LR) + threadIdx.x / LR;
+    const int d = 4 * (threadIdx.x % LR);
+    if (threadIdx.x >= 256 / LR * LR || g >= rows) return;
+    float m = -INFINITY;
+    for (int s = 0; s < f.ns; ++s) m = fmaxf(m, f.part_s[(s * rows + g) * 2]);
+    const float mref = m == -INFINITY ? 0.f : m;
+    float l = 0.f, a0 = 0.f, a1 = 0.f, a2 = 0.f, a3 = 0.f;
+    for (int s = 0; s < f.ns; ++s) {
+        const float ls = f.part_s[(s * rows + g) * 2 + 1];
+        const float w = __builtin_amdgcn_exp2f((f.part_s[(s * rows + g) * 2] - mref) * LOG2E);
+        const f32x4 v = *(const f32x4*)(f.part_o + (s * rows + g) * HDP + d);
+        l = fmaf(ls, w, l);
+        a0 = fmaf(v[0], w, a0); a1 = fmaf(v[1], w, a1); a2 = fmaf(v[2], w, a2); a3 = fmaf(v[3], w, a3);
+    }
+    const int bh = (int)(g / p.R), r = (int)(g - (int64_t)bh * p.R), b = bh / p.Hkv, hk = bh - b * p.Hkv;
+    int tok, h;
+    row_of(p, hk, r, tok, h);
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    if (d < p.hd) store4((T*)f.out + b * p.so.b + tok * p.so.l + h * p.so.h + d, a0 * inv, a1 * inv, a2 * inv, a3 * inv);
+    if (f.stat != nullptr && d == 0) {
+        float* st = f.stat + (((int64_t)b * p.H + h) * p.Lq + tok) * 2;
+        st[0] = m;
+        st[1] = l;
+    }
+}
+
+// How a launch is cut: row blocks, and splits of the keys where the row blocks alone leave CUs idle.
+struct FwdPlan { bool few; int hdp, nrb, ns; int64_t part_bytes; };
+FwdPlan plan_fwd(const MarsCrossAttn* a) {
+    FwdPlan pl;
+    const int64_t R = (int64_t)(a->H / a->Hkv) * a->Lq;
+    pl.hdp = (a->hd + 31) / 32 * 32;
+    pl.few = R <= 32;
+    pl.nrb = (int)(pl.few ? 1 : (R + 127) / 128);
+    const int64_t blocks = (int64_t)a->B * a->Hkv * pl.nrb;
+    const int tiles = (a->Lk + 63) / 64;
+    pl.ns = 1;
+    if (blocks < 256) {
+        const int64_t want = (512 + blocks - 1) / blocks;
+        const int most = pl.few ? (tiles + 3) / 4 : (tiles + 1) / 2;             // at least two tiles a wave
+        pl.ns = (int)(want < most ? want : most);
+        if (pl.ns < 1) pl.ns = 1;
+    }
+    pl.part_bytes = pl.ns > 1 ? (int64_t)pl.ns * a->B * a->Hkv * R * (pl.hdp + 2) * 4 : 0;
+    return pl;
+}
+
+template <typename T, int HDP> int launch_fwd(const Fwd& f, bool few, hipStream_t s) {
+    const int64_t blocks = (int64_t)f.p.B * f.p.Hkv * f.nrb * f.ns;
+    MARS_CHECK(blocks * 256 < (1ll << 32), "cross_attn: %lld workgroups are more than a launch takes", (long long)blocks);
+    const dim3 grid((unsigned)blocks), block(256);
+    if (f.p.bias != nullptr) {
+        if (few) hipLaunchKernelGGL((cross_fwd_kernel<T, HDP, true, true>), grid, block, 0, s, f);
+        else hipLaunchKernelGGL((cross_fwd_kernel<T, HDP, true, false>), grid, block, 0, s, f);
+    } else {
+        if (few) hipLaunchKernelGGL((cross_fwd_kernel<T, HDP, false, true>), grid, block, 0, s, f);
+        else hipLaunchKernelGGL((cross_fwd_kernel<T, HDP, false, false>), grid, block, 0, s, f);
+    }
+    MARS_LAUNCH_CHECK();
+    if (f.ns > 1) {
+        const int64_t rows = (int64_t)f.p.B * f.p.Hkv * f.p.R, per = 256 / (HDP / 4);
+        hipLaunchKernelGGL((cross_join_kernel<T, HDP>), dim3((unsigned)((rows + per - 1) / per)), block, 0, s, f);
+        MARS_LAUNCH_CHECK();
+    }
+    return 0;
+}
+
+template <typename T> int launch_fwd_hd(const Fwd& f, const FwdPlan& pl, hipStream_t s) {
+    switch (pl.hdp) {
+        case 32: return launch_fwd<T, 32>(f, pl.few, s);
+        case 64: return launch_fwd<T, 64>(f, pl.few, s);
+        case 96: return launch_fwd<T, 96>(f, pl.few, s);
+        default: return launch_fwd<T, 128>(f, pl.few, s);
+    }
+}
+
+int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
+
+}  // namespace
+
+// ------------------------------------------------------------------------------------------------ host side, shared with the backward
+static bool rows_ok(const void* ptr, const int64_t* st, int es) {
+    return ((uintptr_t)ptr % 16 == 0) && (st[0] * es) % 16 == 0 && (st[1] * es) % 16 == 0 && (st[2] * es) % 16 == 0;
+}
+
+int check(const MarsCrossAttn* a, bool backward) {
+    const char* what = backward ? "cross_attn_bwd" : "cross_attn";
+    MARS_CHECK(a && a->q && a->k && a->v && a->out, "%s: null pointer", what);
+    MARS_CHECK(a->dtype == 0 || a->dtype == 1, "%s: dtype %d", what, a->dtype);
+    const int es = a->dtype == 1 ? 2 : 4;
+    MARS_CHECK(a->B > 0 && a->Lq > 0 && a->Lk > 0 && a->H > 0 && a->Hkv > 0, "%s: bad shape B=%d Lq=%d Lk=%d H=%d Hkv=%d", what, a->B, a->Lq, a->Lk,
+               a->H, a->Hkv);
+    MARS_CHECK(a->H % a->Hkv == 0, "%s: %d query heads are no multiple of %d key heads", what, a->H, a->Hkv);
+    MARS_CHECK(a->hd > 0 && a->hd <= 128 && (a->hd * es) % 16 == 0, "%s: head dim %d (up to 128, a multiple of 16 bytes)", what, a->hd);
+    MARS_CHECK((int64_t)(a->H / a->Hkv) * a->Lq < (1ll << 30) && a->Lk < (1 << 30), "%s: too many rows", what);
+    MARS_CHECK((int64_t)a->B * a->H < (1ll << 30), "%s: too many heads", what);
+    MARS_CHECK(a->scale > 0.f && a->scale < INFINITY, "%s: scale must be positive and finite", what);
+    MARS_CHECK(rows_ok(a->q, a->q_s, es) && rows_ok(a->k, a->k_s, es) && rows_ok(a->v, a->v_s, es) && rows_ok(a->out, a->out_s, es),
+               "%s: rows must be 16-byte aligned", what);
+    if (backward) {
+        MARS_CHECK(a->stat && a->dout && a->dq && a->dk && a->dv, "%s: null pointer", what);
+        MARS_CHECK(rows_ok(a->dout, a->dout_s, es) && rows_ok(a->dq, a->dq_s, es) && rows_ok(a->dk, a->dk_s, es) && rows_ok(a->dv, a->dv_s, es),
+                   "%s: rows must be 16-byte aligned", what);
+        MARS_CHECK(a->dbias == nullptr || a->bias != nullptr, "%s: a gradient of a bias that is not there", what);
+    }
+    return 0;
+}
+
+static Strides st3(const int64_t* s) { return Strides{s[0], s[1], s[2]}; }
+
+void describe(const MarsCrossAttn* a, Prob& p) {
+    p = Prob{};
+    p.q = a->q; p.k = a->k; p.v = a->v; p.out = a->out; p.dout = a->dout;
+    p.sq = st3(a->q_s); p.sk = st3(a->k_s); p.sv = st3(a->v_s); p.so = st3(a->out_s); p.sdo = st3(a->dout_s);
+    p.bias = a->bias; p.bias_h = a->bias_s[0]; p.bias_l = a->bias_s[1];
+    p.stat = a->stat;
+    p.B = a->B; p.Lq = a->Lq; p.Lk = a->Lk; p.H = a->H; p.Hkv = a->Hkv; p.hd = a->hd;
+    p.grp = a->H / a->Hkv;
+    p.R = p.grp * a->Lq;
+    p.scale = a->scale;
+    p.cnt = a->kv_len;
+}
+
+int64_t key_ws_bytes(const MarsCrossAttn* a) { return a->mask ? align256((int64_t)a->B * a->Lk * 4) + align256((int64_t)a->B * 4) : 0; }
+
+int prepare_keys(const MarsCrossAttn* a, Prob& p, int32_t* ws, hipStream_t s) {
+    if (a->mask == nullptr) return 0;
+    int32_t* cnt = (int32_t*)((char*)ws + align256((int64_t)a->B * a->Lk * 4));
+    hipLaunchKernelGGL(list_keys_kernel, dim3((unsigned)a->B), dim3(1024), 0, s, a->mask, a->kv_len, a->Lk, ws, cnt);
+    MARS_LAUNCH_CHECK();
+    p.idx = ws;
+    p.cnt = cnt;
+    return 0;
+}
+
+int64_t bwd_ws_bytes(const MarsCrossAttn* a);
+
+}  // namespace xattn
+
+extern "C" int64_t marship_cross_attn_ws(const MarsCrossAttn* a, int backward) {
+    if (a == nullptr || a->B <= 0 || a->Lq <= 0 || a->Lk <= 0 || a->H <= 0 || a->Hkv <= 0 || a->hd <= 0) return 0;
+    const int64_t keys = xattn::key_ws_bytes(a);
+    if (backward) return keys + xattn::bwd_ws_bytes(a);
+    return keys + xattn::align256(xattn::plan_fwd(a).part_bytes);
+}
+
+extern "C" int marship_cross_attn(const MarsCrossAttn* a, void* stream) {
+    using namespace xattn;
+    if (const int rc = check(a, false)) return rc;
+    const int64_t need = marship_cross_attn_ws(a, 0);
+    MARS_CHECK(need == 0 || (a->ws != nullptr && (uintptr_t)a->ws % 16 == 0 && a->ws_bytes >= need), "cross_attn: workspace of %lld bytes, %lld needed",
+               (long long)a->ws_bytes, (long long)need);
+    hipStream_t s = (hipStream_t)stream;
+    Fwd f{};
+    describe(a, f.p);
+    if (const int rc = prepare_keys(a, f.p, (int32_t*)a->ws, s)) return rc;
+    const FwdPlan pl = plan_fwd(a);
+    f.out = a->out;
+    f.stat = a->stat;
+    f.nrb = pl.nrb;
+    f.ns = pl.ns;
+    if (pl.ns > 1) {
+        const int64_t rows = (int64_t)a->B * a->Hkv * f.p.R;
+        f.part_o = (float*)((char*)a->ws + key_ws_bytes(a));
+        f.part_s = f.part_o + pl.ns * rows * pl.hdp;
+    }
+    return a->dtype == 1 ? launch_fwd_hd<__bf16>(f, pl, s) : launch_fwd_hd<float>(f, pl, s);
+}

@@ -1,0 +1,514 @@
+// Gradients of the attention between two token sets (attention_cross.hip).  With P the softmax, recomputed tile by tile from
+// the row statistics of the forward pass:
+//
+//   D_i = dO_i . O_i     dP = dO V^T     dS = P (dP - D)     dV = P^T dO     dQ = scale dS K     dK = scale dS^T Q     dbias = sum_b dS
+//
+// Three passes, none with atomics, so that every sum has one order:
+//   queries  a wave owns 32 query rows and walks the keys: S^T = K Q^T and dP^T = V dO^T with the query as lane column, dS^T is the
+//            operand of dQ^T += K^T dS^T.  It also makes D and leaves the row values for the other passes, 32 rows a block.
+//   keys     a wave owns 32 keys and walks the query rows of every head that shares them: S = Q K^T, dP = dO V^T with the key as
+//            lane column; P and dS are the operands of dV^T += dO^T P and dK^T += Q^T dS.
+//   bias     (only where its gradient is asked for) a wave owns a 32 x 64 piece of one head's scores and walks the batch.
+// Recomputing S and dP in each pass costs 2 of 7 products more than one pass over all would, but that one would add into dQ from
+// every key block: atomics, in an order that changes.
+#include "attention_cross.h"
+
+namespace xattn {
+
+int64_t bwd_ws_bytes(const MarsCrossAttn* a);
+
+namespace {
+
+// Row values of 32 query rows: 128 floats - [0, 32) offset of the exponent, [32, 64) factor of the exponential (bias only), [64, 96) D.
+// Without a bias P = 2^(c2 s - offset) with offset = log2(e) maximum + log2(sum).  With one, P = 2^((s - offset) log2 e) factor with offset = maximum
+// and factor = 1 / sum: where the mask is the type's lowest value the sum's logarithm would be lost in the maximum.
+// Rows that do not exist or have no key: P = 0.
+constexpr int RSB = 128;
+
+struct Bwd {
+    Prob p;
+    void *dq, *dk, *dv;
+    Strides sdq, sdk, sdv;
+    float* dbias;
+    int64_t dbias_h, dbias_l;
+    const uint8_t* mask;
+    const int32_t* kv_len;
+    float* rows;                     // [B Hkv][nrb * 4][RSB]
+    float *part_q, *part_k, *part_v; // [ns][..][HDP] partial sums, where a pass is split
+    int nrb, nsq;                    // query pass: blocks of 128 rows, splits of the keys
+    int nkb, nsk;                    // key pass: blocks of 128 keys, splits of the query rows
+};
+
+template <bool BIAS> __device__ __forceinline__ float prob(float s, float c2, float off, float fac) {
+    return BIAS ? __builtin_amdgcn_exp2f((s - off) * LOG2E) * fac : __builtin_amdgcn_exp2f(fmaf(s, c2, -off));
+}
+
+template <typename T, int HDP, bool BIAS>
+__global__ __launch_bounds__(256, (HDP <= 64 && sizeof(T) == 2) ? 2 : 1) void cross_bwd_q_kernel(const Bwd f) {
+    using TL = Tile<T, HDP>;
+    constexpr int KT = (HDP > 64 && sizeof(T) == 4) ? 32 : 64, TB = KT * TL::ROWB, KB = KT / 32, KS = HDP / 16, DM = HDP / 32;
+    __shared__ __attribute__((aligned(16))) unsigned char buf0[2][TB];
+    __shared__ __attribute__((aligned(16))) unsigned char buf1[2][TB];
+    const Prob& p = f.p;
+    const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int bh, blk;
+    place_block(blockIdx.x, p.B * p.Hkv, f.nrb * f.nsq, bh, blk);
+    const int rb = blk % f.nrb, split = blk / f.nrb;
+    const int b = bh / p.Hkv, hk = bh - b * p.Hkv;
+    const int r = rb * 128 + wave * 32 + (lane & 31);
+    const bool row_ok = r < p.R;
+    int l = 0, h = 0;
+    if (row_ok) row_of(p, hk, r, l, h);
+    const int n = key_count(p, b);
+    const int32_t* idx = p.idx == nullptr ? nullptr : p.idx + (int64_t)b * p.Lk;
+    const int hdb = p.hd * (int)sizeof(T);
+    const unsigned char* kbase = (const unsigned char*)row_ptr<T>(p.k, p.sk, b, 0, hk);
+    const unsigned char* vbase = (const unsigned char*)row_ptr<T>(p.v, p.sv, b, 0, hk);
+    const int64_t kl = p.sk.l * (int)sizeof(T), vl = p.sv.l * (int)sizeof(T);
+    auto issue = [&](int t, unsigned char (&dst)[2][TB]) {
+        TL::template fill<KT, 4>(dst[0], wave, lane, hdb, [&](int row) { return kbase + key_row(idx, min(t * KT + row, n - 1)) * kl; });
+        TL::template fill<KT, 4>(dst[1], wave, lane, hdb, [&](int row) { return vbase + key_row(idx, min(t * KT + row, n - 1)) * vl; });
+    };
+    int t0, t1;
+    split_range((n + KT - 1) / KT, split, f.nsq, t0, t1);
+    if (t0 < t1) issue(t0, buf0);
+
+    frag_t<T> qf[KS], dof[KS];
+    const T* qrow = row_ok ? row_ptr<T>(p.q, p.sq, b, l, h) : nullptr;
+    const T* dorow = row_ok ? row_ptr<T>(p.dout, p.sdo, b, l, h) : nullptr;
+    const T* orow = row_ok ? row_ptr<T>(p.out, p.so, b, l, h) : nullptr;
+    const float c2 = p.scale * LOG2E;
+    float D = 0.f, off = BIAS ? 0.f : INFINITY, fac = 0.f;
+    if (row_ok) {
+        const float* st = p.stat + (((int64_t)b * p.H + h) * p.Lq + l) * 2;
+        const float m = st[0], sum = st[1];
+        if (sum != 0.f) {
+            off = BIAS ? m : fmaf(m, LOG2E, __builtin_amdgcn_logf(sum));
+            fac = 1.0f / sum;
+        }
+    }
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+        qf[ks] = load_frag<T>(qrow, ks, hh, p.hd);
+        dof[ks] = load_frag<T>(dorow, ks, hh, p.hd);
+        const frag_t<T> of = load_frag<T>(orow, ks, hh, p.hd);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) D = fmaf((float)dof[ks][e], (float)of[e], D);
+    }
+    D = halves_sum(D);
+    if (split == 0 && hh == 0) {
+        float* rs = f.rows + ((int64_t)bh * f.nrb * 4 + rb * 4 + wave) * RSB + lane;
+        rs[0] = off;
+        rs[32] = fac;
+        rs[64] = D;
+    }
+    const float* brow = BIAS && row_ok ? p.bias + h * p.bias_h + l * p.bias_l : nullptr;
+
+    f32x16 dq[DM];
+#pragma unroll
+    for (int m = 0; m < DM; ++m) dq[m] = zero16();
+    auto tile = [&](int t, const unsigned char* kt, const unsigned char* vt) {
+        const bool ragged = t * KT + KT > n;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+            f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                s = mma(TL::rows(kt, 32 * kb, ks, lane), qf[ks], s);
+                dp = mma(TL::rows(vt, 32 * kb, ks, lane), dof[ks], dp);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int j = t * KT + 32 * kb + acc_row(i, hh);
+                if constexpr (BIAS) s[i] = fmaf(s[i], p.scale, brow != nullptr ? brow[key_row(idx, min(j, n - 1))] : 0.f);
+                float ds = prob<BIAS>(s[i], c2, off, fac) * (dp[i] - D);
+                if (ragged && j >= n) ds = 0.f;
+                s[i] = ds;
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                // (dS of bf16 heads is rounded to bf16 for the matrix instruction, as P is in the forward pass)
+                const frag_t<T> df = pack_step<T>(s, u);
+#pragma unroll
+                for (int m = 0; m < DM; ++m) dq[m] = mma(TL::cols(kt, 32 * kb + 16 * u, m, lane), df, dq[m]);
+            }
+        }
+    };
+    for (int t = t0; t < t1; t += 2) {
+        __syncthreads();
+        if (t + 1 < t1) issue(t + 1, buf1);
+        tile(t, buf0[0], buf0[1]);
+        if (t + 1 < t1) {
+            __syncthreads();
+            if (t + 2 < t1) issue(t + 2, buf0);
+            tile(t + 1, buf1[0], buf1[1]);
+        }
+    }
+    if (!row_ok) return;
+    if (f.nsq > 1) {
+        float* po = f.part_q + (((int64_t)split * p.B * p.Hkv + bh) * p.R + r) * HDP;
+#pragma unroll
+        for (int m = 0; m < DM; ++m)
+#pragma unroll
+            for (int a = 0; a < 4; ++a) *(f32x4*)(po + 32 * m + 8 * a + 4 * hh) = (f32x4){dq[m][4 * a], dq[m][4 * a + 1], dq[m][4 * a + 2], dq[m][4 * a + 3]};
+        return;
+    }
+    T* out = (T*)f.dq + b * f.sdq.b + l * f.sdq.l + h * f.sdq.h;
+#pragma unroll
+    for (int m = 0; m < DM; ++m)
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+            const int d = 32 * m + 8 * a + 4 * hh;
+            if (d < p.hd) store4(out + d, dq[m][4 * a] * p.scale, dq[m][4 * a + 1] * p.scale, dq[m][4 * a + 2] * p.scale, dq[m][4 * a + 3] * p.scale);
+        }
+}
+
+template <typename T, int HDP> struct KeyCfg {
+    static constexpr int QT = HDP <= 64 ? 64 : 32;                  // query rows a tile
+    static constexpr int TB = QT * Tile<T, HDP>::ROWB, RB = QT / 32 * RSB * 4;
+};
+
+template <typename T, int HDP, bool BIAS>
+__global__ __launch_bounds__(256, (HDP <= 64 && sizeof(T) == 2) ? 2 : 1) void cross_bwd_kv_kernel(const Bwd f) {
+    using TL = Tile<T, HDP>;
+    using Cfg = KeyCfg<T, HDP>;
+    constexpr int QT = Cfg::QT, TB = Cfg::TB, KS = HDP / 16, DM = HDP / 32;
+    __shared__ __attribute__((aligned(16))) unsigned char buf0[2 * TB + Cfg::RB];
+    __shared__ __attribute__((aligned(16))) unsigned char buf1[2 * TB + Cfg::RB];
+    const Prob& p = f.p;
+    const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int bh, blk;
+    place_block(blockIdx.x, p.B * p.Hkv, f.nkb * f.nsk, bh, blk);
+    const int kblk = blk % f.nkb, split = blk / f.nkb;
+    const int b = bh / p.Hkv, hk = bh - b * p.Hkv;
+    const int n = key_count(p, b);
+    const int32_t* idx = p.idx == nullptr ? nullptr : p.idx + (int64_t)b * p.Lk;
+    const int pos = kblk * 128 + wave * 32 + (lane & 31);
+    const bool exists = pos < p.Lk, attended = pos < n;
+    const int key = exists ? key_row(idx, pos) : 0;                 // (the list has all Lk keys, those not attended at its end)
+    const int hdb = p.hd * (int)sizeof(T);
+
+    f32x16 dk[DM], dv[DM];
+#pragma unroll
+    for (int m = 0; m < DM; ++m) { dk[m] = zero16(); dv[m] = zero16(); }
+
+    if (kblk * 128 < n) {
+        frag_t<T> kf[KS], vf[KS];
+        const T* krow = attended ? row_ptr<T>(p.k, p.sk, b, key, hk) : nullptr;
+        const T* vrow = attended ? row_ptr<T>(p.v, p.sv, b, key, hk) : nullptr;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) { kf[ks] = load_frag<T>(krow, ks, hh, p.hd); vf[ks] = load_frag<T>(vrow, ks, hh, p.hd); }
+        int t0, t1;
+        split_range((p.R + QT - 1) / QT, split, f.nsk, t0, t1);
+        const float* rows = f.rows + (int64_t)bh * f.nrb * 4 * RSB;
+        auto issue = [&](int t, unsigned char* dst) {
+            auto src = [&](const void* base, const Strides& s, int row) -> const unsigned char* {
+                const int r = t * QT + row;
+                if (r >= p.R) return nullptr;
+                int l, h;
+                row_of(p, hk, r, l, h);
+                return (const unsigned char*)row_ptr<T>(base, s, b, l, h);
+            };
+            TL::template fill<QT, 4>(dst, wave, lane, hdb, [&](int row) { return src(p.q, p.sq, row); });
+            TL::template fill<QT, 4>(dst + TB, wave, lane, hdb, [&](int row) { return src(p.dout, p.sdo, row); });
+            // the row values: 512 bytes a block of 32 rows (they exist up to the next multiple of 128 rows)
+            if (wave == 0 && lane < QT)
+                __builtin_amdgcn_global_load_lds((gbl_ptr_t)(rows + (int64_t)t * (QT / 32) * RSB + 4 * lane), (lds_ptr_t)(dst + 2 * TB), 16, 0, 0);
+        };
+        const float c2 = p.scale * LOG2E;
+        const float* bcol = BIAS && attended ? p.bias + key : nullptr;
+        auto tile = [&](int t, const unsigned char* base) {
+            const unsigned char *qt = base, *dot = base + TB;
+#pragma unroll
+            for (int qb = 0; qb < QT / 32; ++qb) {
+                const float* rs = (const float*)(base + 2 * TB) + qb * RSB;
+                f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    s = mma(TL::rows(qt, 32 * qb, ks, lane), kf[ks], s);
+                    dp = mma(TL::rows(dot, 32 * qb, ks, lane), vf[ks], dp);
+                }
+#pragma unroll
+                for (int a = 0; a < 4; ++a) {
+                    const f32x4 off = *(const f32x4*)(rs + 8 * a + 4 * hh), D = *(const f32x4*)(rs + 64 + 8 * a + 4 * hh);
+                    f32x4 fac = {1.f, 1.f, 1.f, 1.f};
+                    if constexpr (BIAS) fac = *(const f32x4*)(rs + 32 + 8 * a + 4 * hh);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int i = 4 * a + e;
+                        if constexpr (BIAS) {
+                            const int r = t * QT + 32 * qb + acc_row(i, hh);
+                            float bv = 0.f;
+                            if (r < p.R && bcol != nullptr) {
+                                int l, h;
+                                row_of(p, hk, r, l, h);
+                                bv = bcol[h * p.bias_h + l * p.bias_l];
+                            }
+                            s[i] = fmaf(s[i], p.scale, bv);
+                        }
+                        const float pr = prob<BIAS>(s[i], c2, off[e], fac[e]);
+                        s[i] = pr;
+                        dp[i] = pr * (dp[i] - D[e]);
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const frag_t<T> pf = pack_step<T>(s, u), df = pack_step<T>(dp, u);
+#pragma unroll
+                    for (int m = 0; m < DM; ++m) {
+                        dv[m] = mma(TL::cols(dot, 32 * qb + 16 * u, m, lane), pf, dv[m]);
+                        dk[m] = mma(TL::cols(qt, 32 * qb + 16 * u, m, lane), df, dk[m]);
+                    }
+                }
+            }
+        };
+        if (t0 < t1) issue(t0, buf0);
+        for (int t = t0; t < t1; t += 2) {
+            __syncthreads();
+            if (t + 1 < t1) issue(t + 1, buf1);
+            tile(t, buf0);
+            if (t + 1 < t1) {
+                __syncthreads();
+                if (t + 2 < t1) issue(t + 2, buf0);
+                tile(t + 1, buf1);
+            }
+        }
+    }
+    if (!exists) return;
+    if (f.nsk > 1) {
+        const int64_t o = (((int64_t)split * p.B * p.Hkv + bh) * p.Lk + pos) * HDP;
+#pragma unroll
+        for (int m = 0; m < DM; ++m)
+#pragma unroll
+            for (int a = 0; a < 4; ++a) {
+                const int d = 32 * m + 8 * a + 4 * hh;
+                *(f32x4*)(f.part_k + o + d) = (f32x4){dk[m][4 * a], dk[m][4 * a + 1], dk[m][4 * a + 2], dk[m][4 * a + 3]};
+                *(f32x4*)(f.part_v + o + d) = (f32x4){dv[m][4 * a], dv[m][4 * a + 1], dv[m][4 * a + 2], dv[m][4 * a + 3]};
+            }
+        return;
+    }
+    // (a key that is not attended still has its zeros)
+    T* ok = (T*)f.dk + b * f.sdk.b + key * f.sdk.l + hk * f.sdk.h;
+    T* ov = (T*)f.dv + b * f.sdv.b + key * f.sdv.l + hk * f.sdv.h;
+#pragma unroll
+    for (int m = 0; m < DM; ++m)
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+            const int d = 32 * m + 8 * a + 4 * hh;
+            if (d < p.hd) {
+                if (attended) {
+                    store4(ok + d, dk[m][4 * a] * p.scale, dk[m][4 * a + 1] * p.scale, dk[m][4 * a + 2] * p.scale, dk[m][4 * a + 3] * p.scale);
+                    store4(ov + d, dv[m][4 * a], dv[m][4 * a + 1], dv[m][4 * a + 2], dv[m][4 * a + 3]);
+                } else {
+                    store4(ok + d, 0.f, 0.f, 0.f, 0.f);
+                    store4(ov + d, 0.f, 0.f, 0.f, 0.f);
+                }
+            }
+        }
+}
+
+// sums of the splits.  KEYS: rows of dk (y 0) and dv (y 1); otherwise rows of dq
+template <typename T, int HDP, bool KEYS>
+__global__ __launch_bounds__(256) void cross_bwd_sum_kernel(const Bwd f) {
+    constexpr int LR = HDP / 4;
+    const Prob& p = f.p;
+    const int per = KEYS ? p.Lk : p.R, ns = KEYS ? f.nsk : f.nsq;
+    const int64_t rows = (int64_t)p.B * p.Hkv * per;
+    const int64_t g = (int64_t)blockIdx.x * (256 / LR) + threadIdx.x / LR;
+    const int d = 4 * (threadIdx.x % LR);
+    if (threadIdx.x >= 256 / LR * LR || g >= rows || d >= p.hd) return;
+    const int bh = (int)(g / per), r = (int)(g - (int64_t)bh * per), b = bh / p.Hkv, hk = bh - b * p.Hkv;
+    const bool second = KEYS && blockIdx.y == 1;
+    const float* part = KEYS ? (second ? f.part_v : f.part_k) : f.part_q;
+    float a0 = 0.f, a1 = 0.f, a2 = 0.f, a3 = 0.f;
+    if (!KEYS || r < key_count(p, b)) {
+        for (int s = 0; s < ns; ++s) {
+            const f32x4 v = *(const f32x4*)(part + (s * rows + g) * HDP + d);
+            a0 += v[0]; a1 += v[1]; a2 += v[2]; a3 += v[3];
+        }
+        if (!second) { a0 *= p.scale; a1 *= p.scale; a2 *= p.scale; a3 *= p.scale; }
+    }
+    T* o;
+    if constexpr (KEYS) {
+        const int key = key_row(p.idx == nullptr ? nullptr : p.idx + (int64_t)b * p.Lk, r);
+        const Strides& s = second ? f.sdv : f.sdk;
+        o = (T*)(second ? f.dv : f.dk) + b * s.b + key * s.l + hk * s.h;
+    } else {
+        int l, h;
+        row_of(p, hk, r, l, h);
+        o = (T*)f.dq + b * f.sdq.b + l * f.sdq.l + h * f.sdq.h;
+    }
+    store4(o + d, a0, a1, a2, a3);
+}
+
+// dbias[h, i, j] = sum_b dS: grid (key tiles of 64, query blocks of 128, heads); keys are taken where they stand (the lists of attended keys
+// differ from entry to entry), with the key as lane column so that rows of bias and dbias are read and written in whole lines
+template <typename T, int HDP>
+__global__ __launch_bounds__(256, 1) void cross_bwd_bias_kernel(const Bwd f) {
+    using TL = Tile<T, HDP>;
+    constexpr int KT = 64, TB = KT * TL::ROWB, KS = HDP / 16;
+    __shared__ __attribute__((aligned(16))) unsigned char buf[2][TB];
+    const Prob& p = f.p;
+    const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int j0 = blockIdx.x * KT, h = blockIdx.z, hk = h / p.grp, r0 = (h - hk * p.grp) * p.Lq;
+    const int i0 = blockIdx.y * 128 + wave * 32;                    // this wave's query tokens
+    const int hdb = p.hd * (int)sizeof(T);
+    const int l = min(i0 + (lane & 31), p.Lq - 1);
+    f32x16 acc[2] = {zero16(), zero16()};
+    float bias[2][16];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int li = min(i0 + acc_row(i, hh), p.Lq - 1), j = min(j0 + 32 * kb + (lane & 31), p.Lk - 1);
+            bias[kb][i] = p.bias[h * p.bias_h + li * p.bias_l + j];
+        }
+    for (int b = 0; b < p.B; ++b) {
+        const int len = f.kv_len == nullptr ? p.Lk : min(max(f.kv_len[b], 0), p.Lk);
+        if (j0 >= len) continue;                                    // (the same for the whole workgroup)
+        const unsigned char* kbase = (const unsigned char*)row_ptr<T>(p.k, p.sk, b, 0, hk);
+        const unsigned char* vbase = (const unsigned char*)row_ptr<T>(p.v, p.sv, b, 0, hk);
+        __syncthreads();
+        TL::template fill<KT, 4>(buf[0], wave, lane, hdb, [&](int row) { return kbase + min(j0 + row, len - 1) * p.sk.l * (int)sizeof(T); });
+        TL::template fill<KT, 4>(buf[1], wave, lane, hdb, [&](int row) { return vbase + min(j0 + row, len - 1) * p.sv.l * (int)sizeof(T); });
+        frag_t<T> qf[KS], dof[KS];
+        const T* qrow = row_ptr<T>(p.q, p.sq, b, l, h);
+        const T* dorow = row_ptr<T>(p.dout, p.sdo, b, l, h);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) { qf[ks] = load_frag<T>(qrow, ks, hh, p.hd); dof[ks] = load_frag<T>(dorow, ks, hh, p.hd); }
+        float off[16], fac[16], D[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int r = r0 + min(i0 + acc_row(i, hh), p.Lq - 1);
+            const float* rs = f.rows + (((int64_t)b * p.Hkv + hk) * f.nrb * 4 + (r >> 5)) * RSB + (r & 31);
+            off[i] = rs[0];
+            fac[i] = rs[32];
+            D[i] = rs[64];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+            const int j = j0 + 32 * kb + (lane & 31);
+            const bool on = j < len && (f.mask == nullptr || f.mask[(int64_t)b * p.Lk + j] != 0);
+            f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                s = mma(qf[ks], TL::rows(buf[0], 32 * kb, ks, lane), s);
+                dp = mma(dof[ks], TL::rows(buf[1], 32 * kb, ks, lane), dp);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                // (a row that is not attended may hold anything: its values stay in this lane's column and are not used)
+                const float ds = prob<true>(fmaf(s[i], p.scale, bias[kb][i]), 0.f, off[i], fac[i]) * (dp[i] - D[i]);
+                acc[kb][i] += on ? ds : 0.f;
+            }
+        }
+    }
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int li = i0 + acc_row(i, hh), j = j0 + 32 * kb + (lane & 31);
+            if (li < p.Lq && j < p.Lk) f.dbias[h * f.dbias_h + li * f.dbias_l + j] = acc[kb][i];
+        }
+}
+
+struct BwdPlan { int hdp, nrb, nsq, nkb, nsk; int64_t rows_bytes, q_bytes, k_bytes; };
+int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
+
+int splits(int64_t blocks, int64_t most) {
+    if (blocks >= 256) return 1;
+    int64_t ns = (512 + blocks - 1) / blocks;
+    if (ns > most) ns = most;
+    return ns < 1 ? 1 : (int)ns;
+}
+
+BwdPlan plan_bwd(const MarsCrossAttn* a) {
+    BwdPlan pl;
+    const int64_t R = (int64_t)(a->H / a->Hkv) * a->Lq, nbh = (int64_t)a->B * a->Hkv;
+    pl.hdp = (a->hd + 31) / 32 * 32;
+    pl.nrb = (int)((R + 127) / 128);
+    pl.nkb = (a->Lk + 127) / 128;
+    pl.nsq = splits(nbh * pl.nrb, ((int64_t)a->Lk + 127) / 128);
+    pl.nsk = splits(nbh * pl.nkb, (R + 127) / 128);
+    pl.rows_bytes = align256(nbh * pl.nrb * 4 * RSB * 4);
+    pl.q_bytes = pl.nsq > 1 ? align256((int64_t)pl.nsq * nbh * R * pl.hdp * 4) : 0;
+    pl.k_bytes = pl.nsk > 1 ? align256((int64_t)pl.nsk * nbh * a->Lk * pl.hdp * 4) : 0;
+    return pl;
+}
+
+template <typename T, int HDP> int launch_bwd(const Bwd& f, hipStream_t s) {
+    const Prob& p = f.p;
+    const int64_t nbh = (int64_t)p.B * p.Hkv, qb = nbh * f.nrb * f.nsq, kb = nbh * f.nkb * f.nsk, per = 256 / (HDP / 4);
+    MARS_CHECK(qb * 256 < (1ll << 32) && kb * 256 < (1ll << 32), "cross_attn_bwd: more workgroups than a launch takes");
+    const dim3 block(256);
+    if (p.bias != nullptr) hipLaunchKernelGGL((cross_bwd_q_kernel<T, HDP, true>), dim3((unsigned)qb), block, 0, s, f);
+    else hipLaunchKernelGGL((cross_bwd_q_kernel<T, HDP, false>), dim3((unsigned)qb), block, 0, s, f);
+    MARS_LAUNCH_CHECK();
+    if (f.nsq > 1) {
+        hipLaunchKernelGGL((cross_bwd_sum_kernel<T, HDP, false>), dim3((unsigned)((nbh * p.R + per - 1) / per)), block, 0, s, f);
+        MARS_LAUNCH_CHECK();
+    }
+    if (p.bias != nullptr) hipLaunchKernelGGL((cross_bwd_kv_kernel<T, HDP, true>), dim3((unsigned)kb), block, 0, s, f);
+    else hipLaunchKernelGGL((cross_bwd_kv_kernel<T, HDP, false>), dim3((unsigned)kb), block, 0, s, f);
+    MARS_LAUNCH_CHECK();
+    if (f.nsk > 1) {
+        hipLaunchKernelGGL((cross_bwd_sum_kernel<T, HDP, true>), dim3((unsigned)((nbh * p.Lk + per - 1) / per), 2), block, 0, s, f);
+        MARS_LAUNCH_CHECK();
+    }
+    if (f.dbias != nullptr) {
+        const unsigned gy = (unsigned)((p.Lq + 127) / 128);
+        MARS_CHECK(gy <= 65535 && p.H <= 65535, "cross_attn_bwd: more workgroups than a launch takes");
+        hipLaunchKernelGGL((cross_bwd_bias_kernel<T, HDP>), dim3((unsigned)((p.Lk + 63) / 64), gy, (unsigned)p.H), block, 0, s, f);
+        MARS_LAUNCH_CHECK();
+    }
+    return 0;
+}
+
+template <typename T> int launch_bwd_hd(const Bwd& f, int hdp, hipStream_t s) {
+    switch (hdp) {
+        case 32: return launch_bwd<T, 32>(f, s);
+        case 64: return launch_bwd<T, 64>(f, s);
+        case 96: return launch_bwd<T, 96>(f, s);
+        default: return launch_bwd<T, 128>(f, s);
+    }
+}
+
+}  // namespace
+
+int64_t bwd_ws_bytes(const MarsCrossAttn* a) {
+    const BwdPlan pl = plan_bwd(a);
+    return pl.rows_bytes + pl.q_bytes + 2 * pl.k_bytes;
+}
+
+}  // namespace xattn
+
+extern "C" int marship_cross_attn_bwd(const MarsCrossAttn* a, void* stream) {
+    using namespace xattn;
+    if (const int rc = check(a, true)) return rc;
+    const int64_t need = marship_cross_attn_ws(a, 1);
+    MARS_CHECK(a->ws != nullptr && (uintptr_t)a->ws % 16 == 0 && a->ws_bytes >= need, "cross_attn_bwd: workspace of %lld bytes, %lld needed",
+               (long long)a->ws_bytes, (long long)need);
+    hipStream_t s = (hipStream_t)stream;
+    Bwd f{};
+    describe(a, f.p);
+    if (const int rc = prepare_keys(a, f.p, (int32_t*)a->ws, s)) return rc;
+    const BwdPlan pl = plan_bwd(a);
+    char* w = (char*)a->ws + key_ws_bytes(a);
+    f.rows = (float*)w;
+    f.part_q = (float*)(w + pl.rows_bytes);
+    f.part_k = (float*)(w + pl.rows_bytes + pl.q_bytes);
+    f.part_v = (float*)(w + pl.rows_bytes + pl.q_bytes + pl.k_bytes);
+    f.dq = a->dq; f.dk = a->dk; f.dv = a->dv;
+    f.sdq = Strides{a->dq_s[0], a->dq_s[1], a->dq_s[2]};
+    f.sdk = Strides{a->dk_s[0], a->dk_s[1], a->dk_s[2]};
+    f.sdv = Strides{a->dv_s[0], a->dv_s[1], a->dv_s[2]};
+    f.dbias = a->dbias; f.dbias_h = a->dbias_s[0]; f.dbias_l = a->dbias_s[1];
+    f.mask = a->mask;
+    f.kv_len = a->kv_len;
+    f.nrb = pl.nrb; f.nsq = pl.nsq; f.nkb = pl.nkb; f.nsk = pl.nsk;
+    return a->dtype == 1 ? launch_bwd_hd<__bf16>(f, pl.hdp, s) : launch_bwd_hd<float>(f, pl.hdp, s);
+}

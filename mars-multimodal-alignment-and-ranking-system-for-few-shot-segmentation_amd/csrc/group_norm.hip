@@ -1,0 +1,492 @@
+// Group norm with an activation on channels-last maps, and its gradient: x [N, P, C], the C / G channels of a group share the
+// statistics of their P C / G values,
+//
+//   xh = (x - mean) rstd,   y = act(w xh + b);      dz = dy act'(w xh + b),  db = sum dz,  dw = sum dz xh,
+//   dx = rstd (w dz - mean(w dz) - xh mean(w dz xh))        (means over a group)
+//
+// Bound by memory: a thread owns V neighbouring channels (16 bytes of bf16) of every few rows, so a wave reads and writes whole
+// lines, and keeps the channels' parameters in registers.  A map is cut into chunks of rows; the chunks' statistics
+// (count, mean, sum of squares about the mean - no difference of large sums) are joined in a small launch, always in the same order.
+#include <initializer_list>
+#include "common.h"
+#include "../../include/mars_hip.h"
+
+namespace {
+
+constexpr int TH = 256;             // threads a workgroup
+constexpr int KR = 4;               // rows a thread holds at a time
+
+struct Norm {
+    const void* x;
+    int64_t x_n, x_p;
+    const float *w, *b;
+    int N, P, C, G, Cg, V, act;
+    int vpr;                        // vectors a row: C / V
+    int ncb;                        // column blocks of up to TH vectors
+    int chunks, rows;               // chunks of `rows` rows
+};
+
+template <typename T, int V> __device__ __forceinline__ void load_vec(const T* p, float (&v)[V]) {
+    if constexpr (sizeof(T) == 2) {
+        if constexpr (V == 8) { const bf16x8 r = *(const bf16x8*)p;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = (float)r[e];
+        } else if constexpr (V == 4) { const bf16x4 r = *(const bf16x4*)p;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = (float)r[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] = (float)p[e];
+        }
+    } else {
+        if constexpr (V >= 4) {
+#pragma unroll
+            for (int i = 0; i < V / 4; ++i) { const f32x4 r = *(const f32x4*)(p + 4 * i);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[4 * i + e] = r[e];
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] = (float)p[e];
+        }
+    }
+}
+template <typename T, int V> __device__ __forceinline__ void store_vec(T* p, const float (&v)[V]) {
+    if constexpr (sizeof(T) == 2) {
+        if constexpr (V == 8) { bf16x8 r;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) r[e] = (__bf16)v[e];
+            *(bf16x8*)p = r;
+        } else if constexpr (V == 4) { *(bf16x4*)p = (bf16x4){(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) p[e] = (T)v[e];
+        }
+    } else {
+        if constexpr (V >= 4) {
+#pragma unroll
+            for (int i = 0; i < V / 4; ++i) *(f32x4*)(p + 4 * i) = (f32x4){v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) p[e] = (T)v[e];
+        }
+    }
+}
+
+// 0 none, 1 erf GELU, 2 z sigmoid(1.702 z), 3 ReLU, 4 z sigmoid(z)
+__device__ __forceinline__ float act_of(float z, int act) {
+    switch (act) {
+        case 1: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+        case 2: return z / (1.f + expf(-1.702f * z));
+        case 3: return fmaxf(z, 0.f);
+        case 4: return z / (1.f + expf(-z));
+        default: return z;
+    }
+}
+__device__ __forceinline__ float slope_of(float z, int act) {
+    switch (act) {
+        case 1: return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * expf(-0.5f * z * z) * 0.39894228040143268f;
+        case 2: { const float s = 1.f / (1.f + expf(-1.702f * z)); return s + 1.702f * z * s * (1.f - s); }
+        case 3: return z > 0.f ? 1.f : 0.f;
+        case 4: { const float s = 1.f / (1.f + expf(-z)); return s + z * s * (1.f - s); }
+        default: return 1.f;
+    }
+}
+
+// statistics of two sets of values joined: counts, means, sums of squares about the mean
+struct Stat { float n, mean, m2; };
+__device__ __forceinline__ Stat join(const Stat& a, const Stat& b) {
+    const float n = a.n + b.n;
+    if (n == 0.f) return a;
+    const float f = b.n / n, d = b.mean - a.mean;
+    return Stat{n, fmaf(d, f, a.mean), a.m2 + b.m2 + d * d * a.n * f};
+}
+
+// grid (chunks, column blocks, N): part[n][chunk][column block][group] for the groups with a channel in the block
+template <typename T, int V>
+__global__ __launch_bounds__(TH) void norm_stat_kernel(const Norm a, Stat* __restrict__ part) {
+    __shared__ Stat sh[TH];
+    const int tid = threadIdx.x, n = blockIdx.z, cb = blockIdx.y, chunk = blockIdx.x;
+    const int v0 = cb * TH, nv = min(TH, a.vpr - v0);               // this block's vectors
+    const int rl = tid / nv, cv = tid - rl * nv, nrl = TH / nv;     // row lanes
+    const bool on = rl < nrl;
+    Stat st{0.f, 0.f, 0.f};
+    if (on) {
+        const T* base = (const T*)a.x + (int64_t)n * a.x_n + (int64_t)(v0 + cv) * V;
+        const int r1 = min((chunk + 1) * a.rows, a.P);
+        for (int r = chunk * a.rows + rl; r < r1; r += nrl * KR) {
+            float x[KR][V];
+            int cnt = 0;
+#pragma unroll
+            for (int k = 0; k < KR; ++k) {
+                if (r + k * nrl < r1) { load_vec<T, V>(base + (int64_t)(r + k * nrl) * a.x_p, x[k]); ++cnt; }
+            }
+            float s = 0.f, q = 0.f;
+#pragma unroll
+            for (int k = 0; k < KR; ++k)
+                if (k < cnt) {
+#pragma unroll
+                    for (int e = 0; e < V; ++e) s += x[k][e];
+                }
+            const float nn = (float)(cnt * V), mean = s / nn;
+#pragma unroll
+            for (int k = 0; k < KR; ++k)
+                if (k < cnt) {
+#pragma unroll
+                    for (int e = 0; e < V; ++e) q = fmaf(x[k][e] - mean, x[k][e] - mean, q);
+                }
+            st = join(st, Stat{nn, mean, q});
+        }
+    }
+    sh[tid] = st;
+    __syncthreads();
+    // row lanes, pairwise
+    for (int s = 1; s < nrl; s *= 2) {
+        if (on && rl % (2 * s) == 0 && rl + s < nrl) sh[tid] = join(sh[tid], sh[tid + s * nv]);
+        __syncthreads();
+    }
+    // the vectors of a group, pairwise (a group may begin or end outside the block)
+    const int cgv = a.Cg / V, g = (v0 + cv) / cgv, first = max(g * cgv - v0, 0), last = min((g + 1) * cgv - v0, nv), i = cv - first;
+    for (int s = 1; s < cgv && s < nv; s *= 2) {
+        if (rl == 0 && i % (2 * s) == 0 && cv + s < last) sh[cv] = join(sh[cv], sh[cv + s]);
+        __syncthreads();
+    }
+    if (rl == 0 && i == 0) part[(((int64_t)n * a.chunks + chunk) * a.ncb + cb) * a.G + g] = sh[cv];
+}
+
+// one wave a (n, group): mean and rstd from the chunks
+__global__ __launch_bounds__(64) void norm_join_kernel(const Norm a, const Stat* __restrict__ part, float eps, float* __restrict__ stat) {
+    const int g = blockIdx.x, n = blockIdx.y, lane = threadIdx.x;
+    const int per = TH * a.V, cb0 = g * a.Cg / per, cb1 = ((g + 1) * a.Cg - 1) / per;
+    Stat st{0.f, 0.f, 0.f};
+    for (int c = lane; c < a.chunks; c += 64)
+        for (int cb = cb0; cb <= cb1; ++cb) st = join(st, part[(((int64_t)n * a.chunks + c) * a.ncb + cb) * a.G + g]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        const Stat other{__shfl_xor(st.n, o, 64), __shfl_xor(st.mean, o, 64), __shfl_xor(st.m2, o, 64)};
+        st = (lane & o) ? join(other, st) : join(st, other);
+    }
+    if (lane == 0) {
+        float* s = stat + ((int64_t)n * a.G + g) * 2;
+        s[0] = st.mean;
+        s[1] = 1.0f / sqrtf(st.m2 / st.n + eps);
+    }
+}
+
+template <typename TI, typename TO, int V>
+__global__ __launch_bounds__(TH) void norm_apply_kernel(const Norm a, const float* __restrict__ stat, TO* __restrict__ out, int64_t o_n, int64_t o_p) {
+    const int tid = threadIdx.x, n = blockIdx.z, cb = blockIdx.y, chunk = blockIdx.x;
+    const int v0 = cb * TH, nv = min(TH, a.vpr - v0), rl = tid / nv, cv = tid - rl * nv, nrl = TH / nv;
+    if (rl >= nrl) return;
+    const int c = (v0 + cv) * V, g = c / a.Cg;
+    const float mean = stat[((int64_t)n * a.G + g) * 2], rstd = stat[((int64_t)n * a.G + g) * 2 + 1];
+    float w[V], b[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) { w[e] = a.w[c + e] * rstd; b[e] = a.b[c + e]; }
+    const TI* xp = (const TI*)a.x + (int64_t)n * a.x_n + c;
+    TO* op = out + (int64_t)n * o_n + c;
+    const int r1 = min((chunk + 1) * a.rows, a.P);
+    for (int r = chunk * a.rows + rl; r < r1; r += nrl * KR) {
+        float x[KR][V];
+#pragma unroll
+        for (int k = 0; k < KR; ++k)
+            if (r + k * nrl < r1) load_vec<TI, V>(xp + (int64_t)(r + k * nrl) * a.x_p, x[k]);
+#pragma unroll
+        for (int k = 0; k < KR; ++k)
+            if (r + k * nrl < r1) {
+                float y[V];
+#pragma unroll
+                for (int e = 0; e < V; ++e) y[e] = act_of(fmaf(x[k][e] - mean, w[e], b[e]), a.act);
+                store_vec<TO, V>(op + (int64_t)(r + k * nrl) * o_p, y);
+            }
+    }
+}
+
+struct NormBwd {
+    const void* dy;
+    int64_t dy_n, dy_p;
+    void* dx;
+    int64_t dx_n, dx_p;
+    const float* stat;
+    float *part, *sums;             // [N][chunks][C][2], [N][C][2]: sums of dz and dz xh
+    float *dw, *db;
+};
+
+// grid (chunks, column blocks, N): sums of dz and dz xh per channel of a chunk
+template <typename TX, typename TY, int V>
+__global__ __launch_bounds__(TH) void norm_bwd_sum_kernel(const Norm a, const NormBwd d) {
+    __shared__ float sh[TH][2 * V + 1];
+    const int tid = threadIdx.x, n = blockIdx.z, cb = blockIdx.y, chunk = blockIdx.x;
+    const int v0 = cb * TH, nv = min(TH, a.vpr - v0), rl = tid / nv, cv = tid - rl * nv, nrl = TH / nv;
+    float s1[V], s2[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) s1[e] = s2[e] = 0.f;
+    const int c = (v0 + cv) * V;
+    if (rl < nrl) {
+        const int g = c / a.Cg;
+        const float mean = d.stat[((int64_t)n * a.G + g) * 2], rstd = d.stat[((int64_t)n * a.G + g) * 2 + 1];
+        float w[V], b[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) { w[e] = a.w[c + e]; b[e] = a.b[c + e]; }
+        const TX* xp = (const TX*)a.x + (int64_t)n * a.x_n + c;
+        const TY* yp = (const TY*)d.dy + (int64_t)n * d.dy_n + c;
+        const int r1 = min((chunk + 1) * a.rows, a.P);
+        for (int r = chunk * a.rows + rl; r < r1; r += nrl * KR) {
+            float x[KR][V], y[KR][V];
+#pragma unroll
+            for (int k = 0; k < KR; ++k)
+                if (r + k * nrl < r1) {
+                    load_vec<TX, V>(xp + (int64_t)(r + k * nrl) * a.x_p, x[k]);
+                    load_vec<TY, V>(yp + (int64_t)(r + k * nrl) * d.dy_p, y[k]);
+                }
+#pragma unroll
+            for (int k = 0; k < KR; ++k)
+                if (r + k * nrl < r1) {
+#pragma unroll
+                    for (int e = 0; e < V; ++e) {
+                        const float xh = (x[k][e] - mean) * rstd, dz = y[k][e] * slope_of(fmaf(xh, w[e], b[e]), a.act);
+                        s1[e] += dz;
+                        s2[e] = fmaf(dz, xh, s2[e]);
+                    }
+                }
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) { sh[tid][2 * e] = s1[e]; sh[tid][2 * e + 1] = s2[e]; }
+    __syncthreads();
+    for (int i = tid; i < nv * 2 * V; i += TH) {
+        const int v = i / (2 * V), k = i - v * 2 * V;
+        float s = 0.f;
+        for (int r = 0; r < nrl; ++r) s += sh[r * nv + v][k];
+        d.part[(((int64_t)n * a.chunks + chunk) * a.C + (v0 + v) * V) * 2 + k] = s;
+    }
+}
+
+// grid (ceil(2 C / 64), N): the chunks' sums; four waves take the chunks in turn
+__global__ __launch_bounds__(256) void norm_bwd_join_kernel(const Norm a, const NormBwd d) {
+    __shared__ float sh[4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = blockIdx.y, i = blockIdx.x * 64 + lane;
+    float s = 0.f;
+    if (i < 2 * a.C)
+        for (int c = wave; c < a.chunks; c += 4) s += d.part[((int64_t)n * a.chunks + c) * a.C * 2 + i];
+    sh[wave][lane] = s;
+    __syncthreads();
+    if (wave == 0 && i < 2 * a.C) d.sums[(int64_t)n * a.C * 2 + i] = (sh[0][lane] + sh[1][lane]) + (sh[2][lane] + sh[3][lane]);
+}
+
+// grid (chunks + 1, column blocks, N): dx of a chunk; the workgroups behind the last chunk add dw and db up over the batch
+template <typename TX, typename TY, int V>
+__global__ __launch_bounds__(TH) void norm_bwd_apply_kernel(const Norm a, const NormBwd d) {
+    __shared__ float sh[2][TH];
+    const int tid = threadIdx.x, n = blockIdx.z, cb = blockIdx.y, chunk = blockIdx.x;
+    if (chunk == a.chunks) {
+        if (cb != 0) return;
+        const int per = (a.C + a.N - 1) / a.N;
+        for (int c = n * per + tid; c < min((n + 1) * per, a.C); c += TH) {
+            float s1 = 0.f, s2 = 0.f;
+            for (int i = 0; i < a.N; ++i) { s1 += d.sums[((int64_t)i * a.C + c) * 2]; s2 += d.sums[((int64_t)i * a.C + c) * 2 + 1]; }
+            d.db[c] = s1;
+            d.dw[c] = s2;
+        }
+        return;
+    }
+    const int v0 = cb * TH, nv = min(TH, a.vpr - v0), rl = tid / nv, cv = tid - rl * nv, nrl = TH / nv;
+    // means over the groups that have a channel in this block: a wave a group
+    const int g_first = v0 * V / a.Cg, g_last = ((v0 + nv) * V - 1) / a.Cg;
+    const float inv = 1.0f / ((float)a.P * (float)a.Cg);
+    const int g = (rl < nrl) ? (v0 + cv) * V / a.Cg : g_first;
+    float m1 = 0.f, m2 = 0.f;
+    for (int g0 = g_first; g0 <= g_last; g0 += TH) {                // (up to TH groups a step)
+        const int ng = min(TH, g_last - g0 + 1);
+        __syncthreads();
+        for (int q = tid >> 6; q < ng; q += TH / 64) {
+            float t1 = 0.f, t2 = 0.f;
+            for (int c = tid & 63; c < a.Cg; c += 64) {
+                const int ch = (g0 + q) * a.Cg + c;
+                const float w = a.w[ch];
+                t1 = fmaf(w, d.sums[((int64_t)n * a.C + ch) * 2], t1);
+                t2 = fmaf(w, d.sums[((int64_t)n * a.C + ch) * 2 + 1], t2);
+            }
+            t1 = wave_sum(t1);
+            t2 = wave_sum(t2);
+            if ((tid & 63) == 0) { sh[0][q] = t1 * inv; sh[1][q] = t2 * inv; }
+        }
+        __syncthreads();
+        if (g >= g0 && g < g0 + ng) { m1 = sh[0][g - g0]; m2 = sh[1][g - g0]; }
+    }
+    if (rl >= nrl) return;
+    const int c = (v0 + cv) * V;
+    const float mean = d.stat[((int64_t)n * a.G + g) * 2], rstd = d.stat[((int64_t)n * a.G + g) * 2 + 1];
+    float w[V], b[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) { w[e] = a.w[c + e]; b[e] = a.b[c + e]; }
+    const TX* xp = (const TX*)a.x + (int64_t)n * a.x_n + c;
+    const TY* yp = (const TY*)d.dy + (int64_t)n * d.dy_n + c;
+    TX* op = (TX*)d.dx + (int64_t)n * d.dx_n + c;
+    const int r1 = min((chunk + 1) * a.rows, a.P);
+    for (int r = chunk * a.rows + rl; r < r1; r += nrl * KR) {
+        float x[KR][V], y[KR][V];
+#pragma unroll
+        for (int k = 0; k < KR; ++k)
+            if (r + k * nrl < r1) {
+                load_vec<TX, V>(xp + (int64_t)(r + k * nrl) * a.x_p, x[k]);
+                load_vec<TY, V>(yp + (int64_t)(r + k * nrl) * d.dy_p, y[k]);
+            }
+#pragma unroll
+        for (int k = 0; k < KR; ++k)
+            if (r + k * nrl < r1) {
+                float o[V];
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    const float xh = (x[k][e] - mean) * rstd, dz = y[k][e] * slope_of(fmaf(xh, w[e], b[e]), a.act);
+                    o[e] = rstd * (dz * w[e] - m1 - xh * m2);
+                }
+                store_vec<TX, V>(op + (int64_t)(r + k * nrl) * d.dx_p, o);
+            }
+    }
+}
+
+int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
+
+// widest vector that divides a group and keeps every row aligned: 8, 4, 2 or 1 channels
+int vec_width(int Cg, std::initializer_list<uint64_t> addresses, int es) {
+    int V = 8;
+    while (V > 1) {
+        bool ok = Cg % V == 0;
+        const uint64_t al = (uint64_t)(V * es < 16 ? V * es : 16);
+        for (const uint64_t x : addresses) ok = ok && x % al == 0;
+        if (ok) break;
+        V /= 2;
+    }
+    return V;
+}
+
+// chunks of rows: about 1024 workgroups, at least KR rows a thread
+void cut(Norm& a) {
+    a.vpr = a.C / a.V;
+    a.ncb = (a.vpr + TH - 1) / TH;
+    const int nrl = TH / (a.vpr < TH ? a.vpr : TH), least = nrl * KR;
+    const int64_t want = 1024 / ((int64_t)a.N * a.ncb) + 1;
+    int64_t rows = (a.P + want - 1) / want;
+    rows = (rows + least - 1) / least * least;
+    a.rows = (int)rows;
+    a.chunks = (int)((a.P + rows - 1) / rows);
+}
+
+int norm_check(const char* what, int N, int P, int C, int G, int act, int dt_a, int dt_b) {
+    MARS_CHECK(N > 0 && P > 0 && C > 0 && G > 0 && N <= 65535 && C < (1 << 24) && P < (1 << 30), "%s: bad shape N=%d P=%d C=%d", what, N, P, C);
+    MARS_CHECK(C % G == 0, "%s: %d channels do not divide into %d groups", what, C, G);
+    MARS_CHECK(act >= 0 && act <= 4, "%s: activation %d", what, act);
+    MARS_CHECK((dt_a == 0 || dt_a == 1) && (dt_b == 0 || dt_b == 1), "%s: dtype", what);
+    return 0;
+}
+
+#define MARS_NORM_V(F, TA, TB)           \
+    switch (a.V) {                       \
+        case 8: F(TA, TB, 8); break;     \
+        case 4: F(TA, TB, 4); break;     \
+        case 2: F(TA, TB, 2); break;     \
+        default: F(TA, TB, 1); break;    \
+    }
+#define MARS_NORM_T(F)                                                                  \
+    if (dx_t == 1) { if (dy_t == 1) { MARS_NORM_V(F, __bf16, __bf16) } else { MARS_NORM_V(F, __bf16, float) } } \
+    else { if (dy_t == 1) { MARS_NORM_V(F, float, __bf16) } else { MARS_NORM_V(F, float, float) } }
+
+// workspace of the forward call, whatever vector width its addresses allow
+int64_t fwd_ws(int N, int P, int C, int G) {
+    int64_t most = 0;
+    for (int V = 1; V <= 8; V *= 2) {
+        if ((C / G) % V) continue;
+        Norm a{};
+        a.N = N; a.P = P; a.C = C; a.V = V;
+        cut(a);
+        const int64_t b = (int64_t)N * a.chunks * a.ncb * G * (int64_t)sizeof(Stat);
+        if (b > most) most = b;
+    }
+    return align256(most) + align256((int64_t)N * G * 8);
+}
+int64_t bwd_ws(int N, int P, int C, int G) {
+    int64_t most = 0;
+    for (int V = 1; V <= 8; V *= 2) {
+        if ((C / G) % V) continue;
+        Norm a{};
+        a.N = N; a.P = P; a.C = C; a.V = V;
+        cut(a);
+        const int64_t b = (int64_t)N * a.chunks * C * 8;
+        if (b > most) most = b;
+    }
+    return align256(most) + align256((int64_t)N * C * 8);
+}
+
+}  // namespace
+
+extern "C" int64_t marship_group_norm_act_ws(int N, int P, int C, int G, int backward) {
+    if (N <= 0 || P <= 0 || C <= 0 || G <= 0 || C % G) return 0;
+    return backward ? bwd_ws(N, P, C, G) : fwd_ws(N, P, C, G);
+}
+
+extern "C" int marship_group_norm_act(const void* x, int64_t x_n, int64_t x_p, const float* w, const float* b, void* out, int64_t o_n, int64_t o_p, int N, int P,
+                                      int C, int G, float eps, int act, int x_dtype, int out_dtype, float* stat, void* ws, int64_t ws_bytes, void* stream) {
+    MARS_CHECK(x && w && b && out, "group_norm_act: null pointer");
+    if (const int rc = norm_check("group_norm_act", N, P, C, G, act, x_dtype, out_dtype)) return rc;
+    MARS_CHECK(eps >= 0.f, "group_norm_act: eps");
+    const int64_t need = fwd_ws(N, P, C, G);
+    MARS_CHECK(ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= need, "group_norm_act: workspace of %lld bytes, %lld needed", (long long)ws_bytes, (long long)need);
+    const int xe = x_dtype == 1 ? 2 : 4, oe = out_dtype == 1 ? 2 : 4;
+    Norm a{};
+    a.x = x; a.x_n = x_n; a.x_p = x_p; a.w = w; a.b = b;
+    a.N = N; a.P = P; a.C = C; a.G = G; a.Cg = C / G; a.act = act;
+    const int vx = vec_width(a.Cg, {(uint64_t)x, (uint64_t)(x_n * xe), (uint64_t)(x_p * xe)}, xe);
+    const int vo = vec_width(a.Cg, {(uint64_t)out, (uint64_t)(o_n * oe), (uint64_t)(o_p * oe)}, oe);
+    a.V = vx < vo ? vx : vo;
+    cut(a);
+    MARS_CHECK((int64_t)a.chunks < (1 << 23) && a.ncb <= 65535 && G < (1 << 23), "group_norm_act: more workgroups than a launch takes");
+    hipStream_t s = (hipStream_t)stream;
+    Stat* part = (Stat*)ws;
+    float* st = stat != nullptr ? stat : (float*)((char*)ws + (need - align256((int64_t)N * G * 8)));
+    const dim3 grid((unsigned)a.chunks, (unsigned)a.ncb, (unsigned)N);
+    const int dx_t = x_dtype, dy_t = out_dtype;
+#define MARS_STAT(TA, TB, VV) hipLaunchKernelGGL((norm_stat_kernel<TA, VV>), grid, dim3(TH), 0, s, a, part)
+    if (dx_t == 1) { MARS_NORM_V(MARS_STAT, __bf16, __bf16) } else { MARS_NORM_V(MARS_STAT, float, float) }
+    MARS_LAUNCH_CHECK();
+    hipLaunchKernelGGL(norm_join_kernel, dim3((unsigned)G, (unsigned)N), dim3(64), 0, s, a, part, eps, st);
+    MARS_LAUNCH_CHECK();
+#define MARS_APPLY(TA, TB, VV) hipLaunchKernelGGL((norm_apply_kernel<TA, TB, VV>), grid, dim3(TH), 0, s, a, st, (TB*)out, o_n, o_p)
+    MARS_NORM_T(MARS_APPLY)
+    MARS_LAUNCH_CHECK();
+    return 0;
+}
+
+extern "C" int marship_group_norm_act_bwd(const void* x, int64_t x_n, int64_t x_p, const float* w, const float* b, const float* stat, const void* dy, int64_t dy_n,
+                                          int64_t dy_p, void* dx, int64_t dx_n, int64_t dx_p, float* dw, float* db, int N, int P, int C, int G, int act,
+                                          int x_dtype, int dy_dtype, void* ws, int64_t ws_bytes, void* stream) {
+    MARS_CHECK(x && w && b && stat && dy && dx && dw && db, "group_norm_act_bwd: null pointer");
+    if (const int rc = norm_check("group_norm_act_bwd", N, P, C, G, act, x_dtype, dy_dtype)) return rc;
+    const int64_t need = bwd_ws(N, P, C, G);
+    MARS_CHECK(ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= need, "group_norm_act_bwd: workspace of %lld bytes, %lld needed", (long long)ws_bytes, (long long)need);
+    const int xe = x_dtype == 1 ? 2 : 4, ye = dy_dtype == 1 ? 2 : 4;
+    Norm a{};
+    a.x = x; a.x_n = x_n; a.x_p = x_p; a.w = w; a.b = b;
+    a.N = N; a.P = P; a.C = C; a.G = G; a.Cg = C / G; a.act = act;
+    const int vx = vec_width(a.Cg, {(uint64_t)x, (uint64_t)(x_n * xe), (uint64_t)(x_p * xe), (uint64_t)dx, (uint64_t)(dx_n * xe), (uint64_t)(dx_p * xe)}, xe);
+    const int vy = vec_width(a.Cg, {(uint64_t)dy, (uint64_t)(dy_n * ye), (uint64_t)(dy_p * ye)}, ye);
+    a.V = vx < vy ? vx : vy;
+    cut(a);
+    MARS_CHECK((int64_t)a.chunks < (1 << 23) && a.ncb <= 65535, "group_norm_act_bwd: more workgroups than a launch takes");
+    NormBwd d{};
+    d.dy = dy; d.dy_n = dy_n; d.dy_p = dy_p; d.dx = dx; d.dx_n = dx_n; d.dx_p = dx_p; d.stat = stat; d.dw = dw; d.db = db;
+    d.part = (float*)ws;
+    d.sums = (float*)((char*)ws + (need - align256((int64_t)N * C * 8)));
+    hipStream_t s = (hipStream_t)stream;
+    const int dx_t = x_dtype, dy_t = dy_dtype;
+    const dim3 grid((unsigned)a.chunks, (unsigned)a.ncb, (unsigned)N), grid1((unsigned)a.chunks + 1, (unsigned)a.ncb, (unsigned)N);
+#define MARS_BSUM(TA, TB, VV) hipLaunchKernelGGL((norm_bwd_sum_kernel<TA, TB, VV>), grid, dim3(TH), 0, s, a, d)
+    MARS_NORM_T(MARS_BSUM)
+    MARS_LAUNCH_CHECK();
+    hipLaunchKernelGGL(norm_bwd_join_kernel, dim3((unsigned)((2 * C + 63) / 64), (unsigned)N), dim3(256), 0, s, a, d);
+    MARS_LAUNCH_CHECK();
+#define MARS_BAPPLY(TA, TB, VV) hipLaunchKernelGGL((norm_bwd_apply_kernel<TA, TB, VV>), grid1, dim3(TH), 0, s, a, d)
+    MARS_NORM_T(MARS_BAPPLY)
+    MARS_LAUNCH_CHECK();
+    return 0;
+}

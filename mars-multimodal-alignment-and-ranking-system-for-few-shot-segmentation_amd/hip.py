@@ -15,7 +15,7 @@ LIB_PATH = os.environ.get("MARS_HIP_LIB") or os.path.join(_HERE, "csrc", "libmar
 HEADER_PATH = os.path.join(os.path.dirname(_HERE), "include", "mars_hip.h")
 
 F32, BF16 = 0, 1
-ACT_NONE, ACT_GELU, ACT_QUICKGELU = 0, 1, 2
+ACT_NONE, ACT_GELU, ACT_QUICKGELU, ACT_RELU, ACT_SILU = 0, 1, 2, 3, 4
 
 
 class MarsAxisTable(Structure):
@@ -34,6 +34,19 @@ class MarsGemm(Structure):
         ("alpha", c_float), ("act", c_int32), ("in_dtype", c_int32), ("out_dtype", c_int32),
         ("ln_copy", c_void_p), ("ldcopy", c_int64), ("ln_part", c_void_p), ("ln_stat", c_void_p), ("ln_colsum", c_void_p),
         ("ln_lo", c_void_p),
+    ]
+
+
+class MarsCrossAttn(Structure):
+    _fields_ = [
+        ("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("out", c_void_p), ("stat", c_void_p), ("bias", c_void_p),
+        ("kv_len", c_void_p), ("mask", c_void_p),
+        ("q_s", c_int64 * 3), ("k_s", c_int64 * 3), ("v_s", c_int64 * 3), ("out_s", c_int64 * 3), ("bias_s", c_int64 * 2),
+        ("B", c_int32), ("Lq", c_int32), ("Lk", c_int32), ("H", c_int32), ("Hkv", c_int32), ("hd", c_int32),
+        ("scale", c_float), ("dtype", c_int32),
+        ("dout", c_void_p), ("dq", c_void_p), ("dk", c_void_p), ("dv", c_void_p), ("dbias", c_void_p),
+        ("dout_s", c_int64 * 3), ("dq_s", c_int64 * 3), ("dk_s", c_int64 * 3), ("dv_s", c_int64 * 3), ("dbias_s", c_int64 * 2),
+        ("ws", c_void_p), ("ws_bytes", c_int64),
     ]
 
 
@@ -115,12 +128,22 @@ _SIGNATURES = {
     "marship_col_mean": [_P, _L, _I, _I, _I, _P, _P],
     "marship_cam_head": [_P, _P, _P, _I, _I, _F, _P, _P, _P],
     "marship_cam_rows": [_P, _L, _P, _I, _I, _I, _P, _P],
+    "marship_cross_attn_ws": [POINTER(MarsCrossAttn), _I],
+    "marship_cross_attn": [POINTER(MarsCrossAttn), _P],
+    "marship_cross_attn_bwd": [POINTER(MarsCrossAttn), _P],
+    "marship_bucket_bias": [_P, _P, _P, _P, _L, _L, _I, _I, _I, _I, _I, _I, _I, _P],
+    "marship_bucket_bias_bwd_ws": [_I, _I, _I, _I, _I, _I],
+    "marship_bucket_bias_bwd": [_P, _L, _L, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _L, _P],
+    "marship_group_norm_act_ws": [_I, _I, _I, _I, _I],
+    "marship_group_norm_act": [_P, _L, _L, _P, _P, _P, _L, _L, _I, _I, _I, _I, _F, _I, _I, _I, _P, _P, _L, _P],
+    "marship_group_norm_act_bwd": [_P, _L, _L, _P, _P, _P, _P, _L, _L, _P, _L, _L, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _L, _P],
     "marshost_emd_scores": [_P, _L, _I, _I, _P, _P, _I, _I, _P, _I],
     "marshost_emd2_uniform": [_P, _I, _I],
     "marship_last_error": [],
     "marship_version": [],
 }
-_RESTYPES = {"marshost_emd2_uniform": c_double, "marship_last_error": c_char_p}
+_RESTYPES = {"marshost_emd2_uniform": c_double, "marship_cross_attn_ws": c_int64, "marship_bucket_bias_bwd_ws": c_int64,
+             "marship_group_norm_act_ws": c_int64, "marship_last_error": c_char_p}
 
 _lib = None
 

@@ -6,13 +6,14 @@ HIP stream to ``libmars_hip.so``.  Nothing here computes with torch.
 """
 from __future__ import annotations
 
+import bisect
 import ctypes
 from typing import Optional
 
 import torch
 
 from . import hip
-from .hip import BF16, F32, MarsGemm
+from .hip import BF16, F32, MarsCrossAttn, MarsGemm
 
 _vp = ctypes.c_void_p
 
@@ -1013,3 +1014,241 @@ def mask_embed(masks: torch.Tensor, G: int, params, eps: float, out: torch.Tenso
     _req(out.dtype == torch.float32 and out.is_contiguous() and out.numel() == B * G * G * C, "mask_embed: out must be f32 [B, G*G, C]")
     hip.check(hip.lib().marship_mask_embed(ptr(masks), B, G, m4, m, C, *[ptr(p) for p in params], float(eps), ptr(out), stream()),
               "marship_mask_embed")
+
+
+# ---------------------------------------------------------------- a trained cross-attention block over patch features
+def _workspace(nbytes: int, device) -> Optional[torch.Tensor]:
+    """A workspace of one call, from torch's caching allocator: ordered on the call's stream, and inside a captured graph's own
+    pool, so that two calls, streams or graphs never share one."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes > 0 else None
+
+
+def _own_elements(t: torch.Tensor, what: str):
+    """An output whose elements share memory (an expanded or overlapping view) would be written by several threads."""
+    end = 1
+    for st, n in sorted((t.stride(d), t.shape[d]) for d in range(t.dim()) if t.shape[d] > 1):
+        _req(st >= end, f"{what}: elements of an output share memory")
+        end = st * (n - 1) + end
+
+
+def _not_an_input(outs, ins, what: str):
+    """No output starts where another operand does (a result written over an operand that is still being read)."""
+    taken = {t.data_ptr() for t in ins if t is not None}
+    for t in outs:
+        if t is not None:
+            _req(t.data_ptr() not in taken, f"{what}: an output lies on another operand")
+            taken.add(t.data_ptr())
+
+
+def _rows16(what: str, **views):
+    for name, t in views.items():
+        es = t.element_size()
+        _req(t.dim() == 4, f"{what}: {name} must be [batch, tokens, heads, head dim]")
+        _req(t.stride(3) == 1 or t.shape[3] == 1, f"{what}: {name}: the elements of a head must be contiguous")
+        _req(t.data_ptr() % 16 == 0 and all((t.stride(d) * es) % 16 == 0 for d in range(3) if t.shape[d] > 1),
+             f"{what}: {name}: rows must be 16-byte aligned")
+
+
+def _strides3(t: torch.Tensor):
+    return (ctypes.c_int64 * 3)(*(t.stride(d) if t.shape[d] > 1 else 0 for d in range(3)))
+
+
+def _cross_args(what, q, k, v, out, stat, scale, kv_len, mask, bias) -> MarsCrossAttn:
+    _dev(q, k, v, out, stat, kv_len, mask, bias)
+    _rows16(what, q=q, k=k, v=v, out=out)
+    _req(q.dtype == k.dtype == v.dtype == out.dtype and q.dtype in (torch.float32, torch.bfloat16), f"{what}: one dtype, f32 or bf16")
+    B, Lq, H, hd = q.shape
+    Lk, Hkv = k.shape[1], k.shape[2]
+    _req(min(B, Lq, H, hd, Lk, Hkv) > 0, f"{what}: empty operand")
+    _req(tuple(k.shape) == (B, Lk, Hkv, hd) and tuple(v.shape) == (B, Lk, Hkv, hd) and out.shape == q.shape, f"{what}: shape mismatch")
+    _req(H % Hkv == 0, f"{what}: {H} query heads are no multiple of {Hkv} key heads")
+    _req(hd <= 128 and (hd * q.element_size()) % 16 == 0, f"{what}: head dim {hd} (up to 128, a multiple of 16 bytes)")
+    a = MarsCrossAttn()
+    if stat is not None:
+        _req(stat.dtype == torch.float32 and stat.is_contiguous() and tuple(stat.shape) == (B, H, Lq, 2), f"{what}: stat must be contiguous f32 [B, H, Lq, 2]")
+        a.stat = stat.data_ptr()
+    if kv_len is not None:
+        _req(kv_len.dtype == torch.int32 and kv_len.is_contiguous() and tuple(kv_len.shape) == (B,), f"{what}: kv_len must be i32 [B]")
+        a.kv_len = kv_len.data_ptr()
+    if mask is not None:
+        _req(mask.dtype in (torch.uint8, torch.bool) and mask.is_contiguous() and tuple(mask.shape) == (B, Lk),
+             f"{what}: mask must be contiguous u8 or bool [B, Lk]")
+        a.mask = mask.data_ptr()
+    if bias is not None:
+        _req(bias.dtype == torch.float32 and tuple(bias.shape) == (H, Lq, Lk) and (bias.stride(2) == 1 or Lk == 1), f"{what}: bias must be f32 [H, Lq, Lk]")
+        a.bias, a.bias_s = bias.data_ptr(), (ctypes.c_int64 * 2)(bias.stride(0), bias.stride(1))
+    scale = hd ** -0.5 if scale is None else float(scale)
+    _req(0.0 < scale < float("inf"), f"{what}: scale must be positive and finite")
+    a.q, a.k, a.v, a.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+    a.q_s, a.k_s, a.v_s, a.out_s = _strides3(q), _strides3(k), _strides3(v), _strides3(out)
+    a.B, a.Lq, a.Lk, a.H, a.Hkv, a.hd, a.scale, a.dtype = B, Lq, Lk, H, Hkv, hd, scale, dt(q)
+    return a
+
+
+def cross_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, *, stat: Optional[torch.Tensor] = None,
+               scale: Optional[float] = None, kv_len: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None,
+               bias: Optional[torch.Tensor] = None):
+    """out = softmax(scale q.k + bias) v: attention of q [B, Lq, H, hd] over k, v [B, Lk, Hkv, hd] (any strides with contiguous heads and
+    16-byte aligned rows; f32 or bf16; hd up to 128; query head h reads key head h // (H // Hkv)).
+
+    ``kv_len`` i32 [B]: keys at or behind it are not attended; ``mask`` u8 or bool [B, Lk]: only keys with a non-zero entry are; what K and V
+    hold at the others is not read.  ``bias`` f32 [H, Lq, Lk], shared by the batch (-inf and the lowest float are allowed).  A row
+    without a key gives zeros.  ``scale`` defaults to hd ** -0.5.  ``stat`` f32 [B, H, Lq, 2] receives what ``cross_attn_bwd`` needs."""
+    a = _cross_args("cross_attn", q, k, v, out, stat, scale, kv_len, mask, bias)
+    _own_elements(out, "cross_attn")
+    _not_an_input((out, stat), (q, k, v, kv_len, mask, bias), "cross_attn")
+    lib = hip.lib()
+    nws = lib.marship_cross_attn_ws(ctypes.byref(a), 0)
+    ws = _workspace(nws, q.device)
+    if ws is not None:
+        a.ws, a.ws_bytes = ws.data_ptr(), nws
+    hip.check(lib.marship_cross_attn(ctypes.byref(a), stream()), "marship_cross_attn")
+
+
+def cross_attn_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, stat: torch.Tensor, dout: torch.Tensor,
+                   dq: torch.Tensor, dk: torch.Tensor, dv: torch.Tensor, *, dbias: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                   kv_len: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None):
+    """Gradients of ``cross_attn`` from its operands, its ``out`` and ``stat`` and the gradient ``dout`` of ``out``: dq, dk, dv (zeros at keys that are
+    not attended) and, where ``dbias`` f32 [H, Lq, Lk] is given, the bias's, summed over the batch.  The same ``scale``, ``kv_len``, ``mask`` and
+    ``bias`` as in the forward call.  Sums have a fixed order: the same call gives the same bits."""
+    a = _cross_args("cross_attn_bwd", q, k, v, out, stat, scale, kv_len, mask, bias)
+    _req(stat is not None, "cross_attn_bwd: stat of the forward call is needed")
+    _dev(dout, dq, dk, dv, dbias)
+    _rows16("cross_attn_bwd", dout=dout, dq=dq, dk=dk, dv=dv)
+    _req(all(t.dtype == q.dtype for t in (dout, dq, dk, dv)), "cross_attn_bwd: one dtype, f32 or bf16")
+    _req(dout.shape == q.shape and dq.shape == q.shape and dk.shape == k.shape and dv.shape == v.shape, "cross_attn_bwd: shape mismatch")
+    if dbias is not None:
+        _req(bias is not None, "cross_attn_bwd: a gradient of a bias that is not there")
+        _req(dbias.dtype == torch.float32 and dbias.shape == bias.shape and (dbias.stride(2) == 1 or dbias.shape[2] == 1),
+             "cross_attn_bwd: dbias must be f32 [H, Lq, Lk]")
+        _own_elements(dbias, "cross_attn_bwd")
+        a.dbias, a.dbias_s = dbias.data_ptr(), (ctypes.c_int64 * 2)(dbias.stride(0), dbias.stride(1))
+    for t in (dq, dk, dv):
+        _own_elements(t, "cross_attn_bwd")
+    _not_an_input((dq, dk, dv, dbias), (q, k, v, out, stat, dout, kv_len, mask, bias), "cross_attn_bwd")
+    a.dout, a.dq, a.dk, a.dv = dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+    a.dout_s, a.dq_s, a.dk_s, a.dv_s = _strides3(dout), _strides3(dq), _strides3(dk), _strides3(dv)
+    lib = hip.lib()
+    nws = lib.marship_cross_attn_ws(ctypes.byref(a), 1)
+    ws = _workspace(nws, q.device)
+    a.ws, a.ws_bytes = ws.data_ptr(), nws
+    hip.check(lib.marship_cross_attn_bwd(ctypes.byref(a), stream()), "marship_cross_attn_bwd")
+
+
+def bucket_map(n_q: int, n_k: int, buckets: int, reach: int, *, offset: int = 0, bidirectional: bool = True) -> torch.Tensor:
+    """The map of one grid axis for ``bucket_bias``: i32 [n_q + n_k - 1] on the CPU, the bucket of every distance d = key - (query + ``offset``), entry
+    (key - query) + n_q - 1.  Of the buckets of a direction (half of ``buckets``, keys behind the query in the upper half; all of them for
+    keys at or before the query where not ``bidirectional``, whose keys behind the query are in bucket 0) the first half hold one distance each and
+    the others share borders that grow geometrically up to ``reach``; distances from there on are in the last.  Whole-number arithmetic: no
+    distance next to a border depends on a rounding."""
+    _req(n_q > 0 and n_k > 0, "bucket_map: empty axis")
+    side = buckets // 2 if bidirectional else buckets
+    near = side // 2
+    _req(near >= 1 and (not bidirectional or buckets % 2 == 0), f"bucket_map: {buckets} buckets are too few, or odd")
+    _req(reach > near, f"bucket_map: reach {reach} must lie behind the {near} distances that have a bucket of their own")
+    steps = side - near
+    # border t of the shared buckets: the smallest n with (n / near) ** steps >= (reach / near) ** t
+    borders, n = [], near
+    for t in range(1, steps):
+        while n ** steps < reach ** t * near ** (steps - t):
+            n += 1
+        borders.append(n)
+    out = torch.empty(n_q + n_k - 1, dtype=torch.int32)
+    for i in range(n_q + n_k - 1):
+        d = i - (n_q - 1) - offset
+        n = abs(d) if bidirectional else max(-d, 0)
+        b = n if n < near else near + bisect.bisect_right(borders, n)
+        out[i] = b + (side if bidirectional and d > 0 else 0)
+    return out
+
+
+def _bias_args(what, table, by, bx, bias, q_grid, k_grid):
+    _dev(table, by, bx, bias)
+    (qh, qw), (kh, kw) = q_grid, k_grid
+    _req(min(qh, qw, kh, kw) > 0, f"{what}: empty grid")
+    _req(table.dim() == 3 and table.is_contiguous() and table.dtype == torch.float32 and table.numel() > 0, f"{what}: table must be contiguous f32 [ny, nx, H]")
+    ny, nx, H = table.shape
+    for name, m, n in (("by", by, qh + kh - 1), ("bx", bx, qw + kw - 1)):
+        _req(m.dtype == torch.int32 and m.is_contiguous() and tuple(m.shape) == (n,), f"{what}: {name} must be contiguous i32 [{n}]")
+    _req(bias.dtype == torch.float32 and tuple(bias.shape) == (H, qh * qw, kh * kw) and (bias.stride(2) == 1 or kh * kw == 1),
+         f"{what}: the bias must be f32 [H, {qh * qw}, {kh * kw}]")
+    _req(bias.shape[1] == 1 or bias.stride(1) >= kh * kw, f"{what}: rows of the bias overlap")
+    s_row = bias.stride(1) if bias.shape[1] > 1 else kh * kw
+    s_head = bias.stride(0) if H > 1 else s_row * qh * qw
+    return ny, nx, H, s_head, s_row
+
+
+def bucket_bias(table: torch.Tensor, by: torch.Tensor, bx: torch.Tensor, out: torch.Tensor, *, q_grid, k_grid):
+    """out[h, (qy, qx), (ky, kx)] = table[by[ky - qy + qh - 1], bx[kx - qx + qw - 1], h]: the learned position bias of query tokens on a grid
+    ``q_grid`` = (qh, qw) and key tokens on ``k_grid`` = (kh, kw), for ``cross_attn``.  table f32 [ny, nx, H]; by, bx i32 on the device, made by ``bucket_map``
+    or by any other rule (an entry outside the table: no bias); a line of tokens is a grid of one row with by = [0].  out f32 [H, qh qw, kh kw], rows may be
+    wider."""
+    ny, nx, H, s_head, s_row = _bias_args("bucket_bias", table, by, bx, out, q_grid, k_grid)
+    _own_elements(out, "bucket_bias")
+    hip.check(hip.lib().marship_bucket_bias(ptr(table), ptr(by), ptr(bx), ptr(out), s_head, s_row, H, *q_grid, *k_grid, ny, nx, stream()),
+              "marship_bucket_bias")
+
+
+def bucket_bias_bwd(dbias: torch.Tensor, by: torch.Tensor, bx: torch.Tensor, dtable: torch.Tensor, *, q_grid, k_grid):
+    """dtable f32 [ny, nx, H] = sums of dbias f32 [H, qh qw, kh kw] over the pairs of each bucket: the gradient of ``bucket_bias``.  Every entry is written; sums
+    have a fixed order."""
+    ny, nx, H, s_head, s_row = _bias_args("bucket_bias_bwd", dtable, by, bx, dbias, q_grid, k_grid)
+    lib = hip.lib()
+    nws = lib.marship_bucket_bias_bwd_ws(H, *q_grid, *k_grid, nx)
+    ws = _workspace(nws, dbias.device)
+    hip.check(lib.marship_bucket_bias_bwd(ptr(dbias), s_head, s_row, ptr(by), ptr(bx), ptr(dtable), H, *q_grid, *k_grid, ny, nx, ptr(ws), nws, stream()),
+              "marship_bucket_bias_bwd")
+
+
+def _norm_args(what, groups, act, w, b, **maps):
+    _dev(w, b, *maps.values())
+    x = maps["x"]
+    _req(x.dim() == 3 and x.numel() > 0, f"{what}: x must be [N, P, C]")
+    N, P, C = x.shape
+    for name, t in maps.items():
+        _req(t.shape == x.shape and t.dtype in (torch.float32, torch.bfloat16) and (t.stride(2) == 1 or C == 1),
+             f"{what}: {name} must be f32 or bf16 [N, P, C] with contiguous channels")
+    _req(groups > 0 and C % groups == 0, f"{what}: {C} channels do not divide into {groups} groups")
+    _req(act in (0, 1, 2, 3, 4), f"{what}: activation {act}")
+    for name, t in (("w", w), ("b", b)):
+        _req(t.dtype == torch.float32 and t.is_contiguous() and tuple(t.shape) == (C,), f"{what}: {name} must be contiguous f32 [C]")
+    return N, P, C
+
+
+def group_norm_act(x: torch.Tensor, w: torch.Tensor, b: torch.Tensor, out: torch.Tensor, groups: int, eps: float, act: int = 0, *,
+                   stat: Optional[torch.Tensor] = None):
+    """out = act(GroupNorm(x)) for channels-last maps x [N, P, C] (P pixels or tokens; rows may be wider than C), f32 or bf16 in and out; act is one of
+    ``hip.ACT_NONE / ACT_GELU / ACT_QUICKGELU / ACT_RELU / ACT_SILU``.  ``stat`` f32 [N, groups, 2] receives mean and 1 / sqrt(var + eps), which
+    ``group_norm_act_bwd`` needs.  out may be x itself."""
+    N, P, C = _norm_args("group_norm_act", groups, act, w, b, x=x, out=out)
+    _own_elements(out, "group_norm_act")
+    _req(eps >= 0.0, "group_norm_act: eps")
+    if stat is not None:
+        _dev(stat)
+        _req(stat.dtype == torch.float32 and stat.is_contiguous() and tuple(stat.shape) == (N, groups, 2), "group_norm_act: stat must be contiguous f32 [N, groups, 2]")
+    lib = hip.lib()
+    nws = lib.marship_group_norm_act_ws(N, P, C, groups, 0)
+    ws = _workspace(nws, x.device)
+    hip.check(lib.marship_group_norm_act(ptr(x), x.stride(0), x.stride(1), ptr(w), ptr(b), ptr(out), out.stride(0), out.stride(1), N, P, C, groups, eps, act,
+                                         dt(x), dt(out), ptr(stat), ptr(ws), nws, stream()), "marship_group_norm_act")
+
+
+def group_norm_act_bwd(x: torch.Tensor, w: torch.Tensor, b: torch.Tensor, stat: torch.Tensor, dy: torch.Tensor, dx: torch.Tensor, dw: torch.Tensor,
+                       db: torch.Tensor, groups: int, act: int = 0):
+    """Gradients of ``group_norm_act``: dx [N, P, C] in x's dtype, dw and db f32 [C], from x, the parameters, the forward call's ``stat`` and the gradient dy of
+    the output.  dx may be dy itself.  Sums have a fixed order."""
+    N, P, C = _norm_args("group_norm_act_bwd", groups, act, w, b, x=x, dy=dy, dx=dx)
+    _req(dx.dtype == x.dtype, "group_norm_act_bwd: dx must have x's dtype")
+    _own_elements(dx, "group_norm_act_bwd")
+    _dev(stat, dw, db)
+    _req(stat.dtype == torch.float32 and stat.is_contiguous() and tuple(stat.shape) == (N, groups, 2),
+         "group_norm_act_bwd: stat must be contiguous f32 [N, groups, 2]")
+    for name, t in (("dw", dw), ("db", db)):
+        _req(t.dtype == torch.float32 and t.is_contiguous() and tuple(t.shape) == (C,), f"group_norm_act_bwd: {name} must be contiguous f32 [C]")
+    _not_an_input((dw, db), (x, w, b, stat, dy, dx), "group_norm_act_bwd")
+    lib = hip.lib()
+    nws = lib.marship_group_norm_act_ws(N, P, C, groups, 1)
+    ws = _workspace(nws, x.device)
+    hip.check(lib.marship_group_norm_act_bwd(ptr(x), x.stride(0), x.stride(1), ptr(w), ptr(b), ptr(stat), ptr(dy), dy.stride(0), dy.stride(1), ptr(dx),
+                                             dx.stride(0), dx.stride(1), ptr(dw), ptr(db), N, P, C, groups, act, dt(x), dt(dy), ptr(ws), nws, stream()),
+              "marship_group_norm_act_bwd")
