@@ -78,24 +78,27 @@ template <typename T, int HDP> struct Tile {
         else if constexpr (LPR % 8 == 0) return (r >> 1) & 7;
         else return (r >> 2) & 3;
     }
-    // rows [0, NR) by NW waves of which this is number w; src(row) gives the row's first byte, or nullptr for a row of zeros; hdb: bytes
-    // of a row that exist (the rest of a row is zeros)
-    template <int NR, int NW, typename F>
-    static __device__ __forceinline__ void fill(unsigned char* dst, int w, int lane, int hdb, F src) {
-        constexpr int PIECES = NR * LPR / 64;
+    // rows [0, NR) by NW waves of which this is number w: fill number i of a lane is 16 bytes of row row_of_fill(i) (FILLS of them)
+    template <int NR, int NW> struct Fill {
+        static constexpr int PIECES = NR * LPR / 64, FILLS = (PIECES + NW - 1) / NW;
         static_assert(NR * LPR % 64 == 0, "a tile is a whole number of 1-KiB pieces");
+        static __device__ __forceinline__ int row_of_fill(int i, int w, int lane) { return ((w + i * NW) * 64 + lane) / LPR; }
+        // at(i): the first byte of fill i's row; hdb: bytes of a row that exist (the rest is zeros).  Straight-line code: a branch or a wait
+        // between two fills would hold up the later ones by a trip to memory
+        template <typename F> static __device__ __forceinline__ void run(unsigned char* dst, int w, int lane, int hdb, F at) {
+            const unsigned char* zeros = (const unsigned char*)&zero_chunk;
 #pragma unroll
-        for (int i = 0; i < (PIECES + NW - 1) / NW; ++i) {
-            const int p = w + i * NW;
-            if (PIECES % NW == 0 || p < PIECES) {
-                const int c = p * 64 + lane, row = c / LPR, slot = c - row * LPR;
-                const int byte = (slot ^ swizzle(row)) * 16;
-                const unsigned char* s = src(row);
-                s = (s != nullptr && byte < hdb) ? s + byte : (const unsigned char*)&zero_chunk;
-                __builtin_amdgcn_global_load_lds((gbl_ptr_t)s, (lds_ptr_t)(dst + p * 1024), 16, 0, 0);
+            for (int i = 0; i < FILLS; ++i) {
+                const int p = w + i * NW;
+                if (PIECES % NW == 0 || p < PIECES) {
+                    const int c = p * 64 + lane, row = c / LPR, slot = c - row * LPR, byte = (slot ^ swizzle(row)) * 16;
+                    const unsigned char* s = at(i) + byte;
+                    s = byte < hdb ? s : zeros;
+                    __builtin_amdgcn_global_load_lds((gbl_ptr_t)s, (lds_ptr_t)(dst + p * 1024), 16, 0, 0);
+                }
             }
         }
-    }
+    };
     // fragment of rows r0 + (lane & 31), contraction step ks over the row's elements
     static __device__ __forceinline__ frag_t<T> rows(const unsigned char* t, int r0, int ks, int lane) {
         const int row = r0 + (lane & 31), hh = lane >> 5, sw = swizzle(row);
@@ -130,6 +133,38 @@ template <typename T, int HDP> struct Tile {
         }
     }
 };
+
+// sixteen bias values of a query row for 32 keys from j0, in the order of an accumulator: keys j0 + acc_row(i).  WHOLE: all 32 keys exist and
+// stand in order, four of them a load (rows of any alignment); otherwise by the list of attended keys, the last one again behind its end
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+template <bool WHOLE> __device__ __forceinline__ void load_bias(float (&v)[16], const float* row, const int32_t* idx, int j0, int n, int hh) {
+    if (row == nullptr) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = 0.f;
+        return;
+    }
+    if (WHOLE && idx == nullptr) {
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+            const f32x4_any x = *(const f32x4_any*)(row + j0 + 8 * a + 4 * hh);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[4 * a + e] = x[e];
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int j = min(j0 + 8 * (i >> 2) + 4 * hh + (i & 3), n - 1);
+        v[i] = row[idx == nullptr ? j : idx[j]];
+    }
+}
+
+// The barrier between a tile's fills and its reads.  A wave's own LDS reads wait for the wave's own fills, but nothing waits for the other
+// waves': each wave drains its fills (vmcnt 0) before it arrives.
+__device__ __forceinline__ void tile_barrier() {
+    __builtin_amdgcn_s_waitcnt(0x0f70);
+    __syncthreads();
+}
 
 // fragment ks of a row in memory (nullptr: zeros); hd: elements of the row that exist, a multiple of 16 bytes
 template <typename T> __device__ __forceinline__ frag_t<T> load_frag(const T* row, int ks, int hh, int hd) {

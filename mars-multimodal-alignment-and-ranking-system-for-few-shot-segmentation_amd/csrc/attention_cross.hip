@@ -11,6 +11,7 @@
 // batch entry, and the fills gather K and V rows through that list.  A support image's foreground is a tenth to
 // a half of its patches, a row costs the same gathered or not (it is at least one 32-byte sector, mostly one or two cache lines),
 // and whatever stands in a masked row - infinities, NaN - is never read.
+#include <type_traits>
 #include "attention_cross.h"
 
 namespace xattn {
@@ -102,13 +103,26 @@ __global__ __launch_bounds__(256, (FwdCfg<T, HDP, FEW>::WPE)) void cross_fwd_ker
     const unsigned char* vbase = (const unsigned char*)row_ptr<T>(p.v, p.sv, b, 0, hk);
     const int64_t kl = p.sk.l * (int)sizeof(T), vl = p.sv.l * (int)sizeof(T);
 
+    // The rows that this thread's fills of a tile take; with a list of attended keys they are looked up a tile ahead, so that no fill
+    // waits for its index.  (Keys behind the last attended one: that one again - their scores are set to -inf, and its row holds
+    // no value that the sums would not see anyway.)
+    constexpr int NW = FEW ? 1 : 4, STEP = FEW ? 4 : 1;
+    using FL = typename TL::template Fill<KT, NW>;
+    const int fw = FEW ? 0 : wave;
+    int rows[FL::FILLS];
+    auto look_up = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < FL::FILLS; ++i) rows[i] = max(min(t * KT + FL::row_of_fill(i, fw, lane), n - 1), 0);
+        if (idx != nullptr && n > 0) {
+#pragma unroll
+            for (int i = 0; i < FL::FILLS; ++i) rows[i] = idx[rows[i]];
+        }
+    };
+    // fills of tile t, whose rows are looked up; then the rows of the next one
     auto issue = [&](int t, unsigned char* dst) {
-        constexpr int NW = FEW ? 1 : 4;
-        const int w = FEW ? 0 : wave;
-        // (keys behind the last attended one: that one again - their scores are set to -inf, and its row holds no value that the
-        // sums would not see anyway)
-        TL::template fill<KT, NW>(dst, w, lane, hdb, [&](int row) { return kbase + key_row(idx, min(t * KT + row, n - 1)) * kl; });
-        TL::template fill<KT, NW>(dst + TB, w, lane, hdb, [&](int row) { return vbase + key_row(idx, min(t * KT + row, n - 1)) * vl; });
+        FL::run(dst, fw, lane, hdb, [&](int i) { return kbase + rows[i] * kl; });
+        FL::run(dst + TB, fw, lane, hdb, [&](int i) { return vbase + rows[i] * vl; });
+        look_up(t + STEP);
     };
 
     f32x16 o[DM];
@@ -120,9 +134,17 @@ __global__ __launch_bounds__(256, (FwdCfg<T, HDP, FEW>::WPE)) void cross_fwd_ker
     // one tile: scores, running maximum, exponentials, products with V.  Without a bias the maximum is of the raw products
     // (scale > 0) and scale and log2 e come with the exponent; with one the scores are kept in natural units, because
     // a mask made of the type's lowest value would overflow in units of log 2.
-    auto tile = [&](int t, const unsigned char* kt, const unsigned char* vt) {
+    // next(): the fills of a later tile, issued behind this tile's bias loads (loads come back in order: the other way round the first use of
+    // the bias would wait for the fills)
+    auto tile_of = [&](auto whole_tag, int t, const unsigned char* kt, const unsigned char* vt, auto next) {
+        constexpr bool WHOLE = decltype(whole_tag)::value;
         f32x16 s[KB];
-        const bool ragged = t * KT + KT > n;
+        float bias[BIAS ? KB : 1][16];
+        if constexpr (BIAS) {
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) load_bias<WHOLE>(bias[kb], brow, idx, t * KT + 32 * kb, n, hh);
+        }
+        next();
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
             s[kb] = zero16();
@@ -130,12 +152,9 @@ __global__ __launch_bounds__(256, (FwdCfg<T, HDP, FEW>::WPE)) void cross_fwd_ker
             for (int ks = 0; ks < KS; ++ks) s[kb] = mma(TL::rows(kt, 32 * kb, ks, lane), qf[ks], s[kb]);
             if constexpr (BIAS) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int j = min(t * KT + 32 * kb + acc_row(i, hh), n - 1);
-                    s[kb][i] = fmaf(s[kb][i], p.scale, brow != nullptr ? brow[key_row(idx, j)] : 0.f);
-                }
+                for (int i = 0; i < 16; ++i) s[kb][i] = fmaf(s[kb][i], p.scale, bias[kb][i]);
             }
-            if (ragged) {
+            if constexpr (!WHOLE) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
                     if (t * KT + 32 * kb + acc_row(i, hh) >= n) s[kb][i] = -INFINITY;
@@ -178,25 +197,29 @@ __global__ __launch_bounds__(256, (FwdCfg<T, HDP, FEW>::WPE)) void cross_fwd_ker
                 for (int m = 0; m < DM; ++m) o[m] = mma(TL::cols(vt, 32 * kb + 16 * u, m, lane), pf, o[m]);
             }
     };
+    auto tile = [&](int t, const unsigned char* kt, const unsigned char* vt, auto next) {
+        if (t * KT + KT <= n) tile_of(std::true_type{}, t, kt, vt, next);
+        else tile_of(std::false_type{}, t, kt, vt, next);
+    };
+    auto nothing = [] {};
 
     if constexpr (!FEW) {
+        look_up(t0);
         if (t0 < t1) issue(t0, buf0[0][0]);
         if constexpr (Cfg::BUFS == 2) {
             for (int t = t0; t < t1; t += 2) {
-                __syncthreads();
-                if (t + 1 < t1) issue(t + 1, buf1[0][0]);
-                tile(t, buf0[0][0], buf0[0][1]);
+                tile_barrier();
+                tile(t, buf0[0][0], buf0[0][1], [&] { if (t + 1 < t1) issue(t + 1, buf1[0][0]); });
                 if (t + 1 < t1) {
-                    __syncthreads();
-                    if (t + 2 < t1) issue(t + 2, buf0[0][0]);
-                    tile(t + 1, buf1[0][0], buf1[0][1]);
+                    tile_barrier();
+                    tile(t + 1, buf1[0][0], buf1[0][1], [&] { if (t + 2 < t1) issue(t + 2, buf0[0][0]); });
                 }
             }
         } else {
             for (int t = t0; t < t1; ++t) {
-                __syncthreads();
-                tile(t, buf0[0][0], buf0[0][1]);
-                __syncthreads();
+                tile_barrier();
+                tile(t, buf0[0][0], buf0[0][1], nothing);
+                tile_barrier();
                 if (t + 1 < t1) issue(t + 1, buf0[0][0]);
             }
         }
@@ -205,22 +228,21 @@ __global__ __launch_bounds__(256, (FwdCfg<T, HDP, FEW>::WPE)) void cross_fwd_ker
         unsigned char* my1 = Cfg::BUFS == 2 ? buf1[Cfg::BUFS == 2 ? cw : 0][0] : my0;
         // waves without a tile skip the loops; a wave's own buffers need its own waits only
         const int first = t0 + wave;
+        look_up(first);
         if (first < t1) issue(first, my0);
         if constexpr (Cfg::BUFS == 2) {
             for (int t = first; t < t1; t += 8) {
                 __builtin_amdgcn_s_waitcnt(0);
-                if (t + 4 < t1) issue(t + 4, my1);
-                tile(t, my0, my0 + TB);
+                tile(t, my0, my0 + TB, [&] { if (t + 4 < t1) issue(t + 4, my1); });
                 if (t + 4 < t1) {
                     __builtin_amdgcn_s_waitcnt(0);
-                    if (t + 8 < t1) issue(t + 8, my0);
-                    tile(t + 4, my1, my1 + TB);
+                    tile(t + 4, my1, my1 + TB, [&] { if (t + 8 < t1) issue(t + 8, my0); });
                 }
             }
         } else {
             for (int t = first; t < t1; t += 4) {
                 __builtin_amdgcn_s_waitcnt(0);
-                tile(t, my0, my0 + TB);
+                tile(t, my0, my0 + TB, nothing);
                 __builtin_amdgcn_s_waitcnt(0);
                 if (t + 4 < t1) issue(t + 4, my0);
             }

@@ -6,11 +6,16 @@
 // Three passes, none with atomics, so that every sum has one order:
 //   queries  a wave owns 32 query rows and walks the keys: S^T = K Q^T and dP^T = V dO^T with the query as lane column, dS^T is the
 //            operand of dQ^T += K^T dS^T.  It also makes D and leaves the row values for the other passes, 32 rows a block.
+//            bf16: the stored O is rounded, and D' = dO . O with it (half a step of each O_d, against a D that is a small difference of
+//            large terms) put 3e-3 into dbias and took dQ from 1.7e-3 to 2.6e-3.  But sum_j P (dP - D') = D - D' exactly: the pass works
+//            with D', adds up e = sum_j dS' in f32 and R = sum_j P_j K_j, and ends with dQ = scale (sum dS' K - e R) and D = D' + e.
+//            One product more in this pass, and no second copy of O in memory.
 //   keys     a wave owns 32 keys and walks the query rows of every head that shares them: S = Q K^T, dP = dO V^T with the key as
 //            lane column; P and dS are the operands of dV^T += dO^T P and dK^T += Q^T dS.
 //   bias     (only where its gradient is asked for) a wave owns a 32 x 64 piece of one head's scores and walks the batch.
 // Recomputing S and dP in each pass costs 2 of 7 products more than one pass over all would, but that one would add into dQ from
 // every key block: atomics, in an order that changes.
+#include <type_traits>
 #include "attention_cross.h"
 
 namespace xattn {
@@ -34,7 +39,8 @@ struct Bwd {
     const uint8_t* mask;
     const int32_t* kv_len;
     float* rows;                     // [B Hkv][nrb * 4][RSB]
-    float *part_q, *part_k, *part_v; // [ns][..][HDP] partial sums, where a pass is split
+    float *part_q, *part_k, *part_v; // [ns][..][HDP] partial sums, where a pass is split (part_q bf16: dS' K, then P K, of a row)
+    float* part_e;                   // [nsq][B Hkv][R]: partial sums of dS'
     int nrb, nsq;                    // query pass: blocks of 128 rows, splits of the keys
     int nkb, nsk;                    // key pass: blocks of 128 keys, splits of the query rows
 };
@@ -66,12 +72,25 @@ __global__ __launch_bounds__(256, (HDP <= 64 && sizeof(T) == 2) ? 2 : 1) void cr
     const unsigned char* kbase = (const unsigned char*)row_ptr<T>(p.k, p.sk, b, 0, hk);
     const unsigned char* vbase = (const unsigned char*)row_ptr<T>(p.v, p.sv, b, 0, hk);
     const int64_t kl = p.sk.l * (int)sizeof(T), vl = p.sv.l * (int)sizeof(T);
+    // rows of a tile's fills: looked up a tile ahead, as in the forward pass
+    using FL = typename TL::template Fill<KT, 4>;
+    int rows[FL::FILLS];
+    auto look_up = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < FL::FILLS; ++i) rows[i] = max(min(t * KT + FL::row_of_fill(i, wave, lane), n - 1), 0);
+        if (idx != nullptr && n > 0) {
+#pragma unroll
+            for (int i = 0; i < FL::FILLS; ++i) rows[i] = idx[rows[i]];
+        }
+    };
     auto issue = [&](int t, unsigned char (&dst)[2][TB]) {
-        TL::template fill<KT, 4>(dst[0], wave, lane, hdb, [&](int row) { return kbase + key_row(idx, min(t * KT + row, n - 1)) * kl; });
-        TL::template fill<KT, 4>(dst[1], wave, lane, hdb, [&](int row) { return vbase + key_row(idx, min(t * KT + row, n - 1)) * vl; });
+        FL::run(dst[0], wave, lane, hdb, [&](int i) { return kbase + rows[i] * kl; });
+        FL::run(dst[1], wave, lane, hdb, [&](int i) { return vbase + rows[i] * vl; });
+        look_up(t + 1);
     };
     int t0, t1;
     split_range((n + KT - 1) / KT, split, f.nsq, t0, t1);
+    look_up(t0);
     if (t0 < t1) issue(t0, buf0);
 
     frag_t<T> qf[KS], dof[KS];
@@ -97,19 +116,23 @@ __global__ __launch_bounds__(256, (HDP <= 64 && sizeof(T) == 2) ? 2 : 1) void cr
         for (int e = 0; e < 8; ++e) D = fmaf((float)dof[ks][e], (float)of[e], D);
     }
     D = halves_sum(D);
-    if (split == 0 && hh == 0) {
-        float* rs = f.rows + ((int64_t)bh * f.nrb * 4 + rb * 4 + wave) * RSB + lane;
-        rs[0] = off;
-        rs[32] = fac;
-        rs[64] = D;
-    }
     const float* brow = BIAS && row_ok ? p.bias + h * p.bias_h + l * p.bias_l : nullptr;
 
-    f32x16 dq[DM];
+    constexpr bool MEND = sizeof(T) == 2;                           // D from a rounded O
+    f32x16 dq[DM], pk[MEND ? DM : 1];
+    float e = 0.f;
 #pragma unroll
     for (int m = 0; m < DM; ++m) dq[m] = zero16();
-    auto tile = [&](int t, const unsigned char* kt, const unsigned char* vt) {
-        const bool ragged = t * KT + KT > n;
+#pragma unroll
+    for (int m = 0; m < (MEND ? DM : 1); ++m) pk[m] = zero16();
+    auto tile_of = [&](auto whole_tag, int t, const unsigned char* kt, const unsigned char* vt, auto next) {
+        constexpr bool WHOLE = decltype(whole_tag)::value;
+        float bias[BIAS ? KB : 1][16];
+        if constexpr (BIAS) {
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) load_bias<WHOLE>(bias[kb], brow, idx, t * KT + 32 * kb, n, hh);
+        }
+        next();
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
             f32x16 s = zero16(), dp = zero16();
@@ -120,38 +143,61 @@ __global__ __launch_bounds__(256, (HDP <= 64 && sizeof(T) == 2) ? 2 : 1) void cr
             }
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const int j = t * KT + 32 * kb + acc_row(i, hh);
-                if constexpr (BIAS) s[i] = fmaf(s[i], p.scale, brow != nullptr ? brow[key_row(idx, min(j, n - 1))] : 0.f);
-                float ds = prob<BIAS>(s[i], c2, off, fac) * (dp[i] - D);
-                if (ragged && j >= n) ds = 0.f;
-                s[i] = ds;
+                if constexpr (BIAS) s[i] = fmaf(s[i], p.scale, bias[kb][i]);
+                float pr = prob<BIAS>(s[i], c2, off, fac);
+                if (!WHOLE && t * KT + 32 * kb + acc_row(i, hh) >= n) pr = 0.f;
+                s[i] = pr;
+                dp[i] = pr * (dp[i] - D);
+                if constexpr (MEND) e += dp[i];
             }
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 // (dS of bf16 heads is rounded to bf16 for the matrix instruction, as P is in the forward pass)
-                const frag_t<T> df = pack_step<T>(s, u);
+                const frag_t<T> df = pack_step<T>(dp, u);
+                frag_t<T> pf = df;
+                if constexpr (MEND) pf = pack_step<T>(s, u);
 #pragma unroll
-                for (int m = 0; m < DM; ++m) dq[m] = mma(TL::cols(kt, 32 * kb + 16 * u, m, lane), df, dq[m]);
+                for (int m = 0; m < DM; ++m) {
+                    const frag_t<T> kc = TL::cols(kt, 32 * kb + 16 * u, m, lane);
+                    dq[m] = mma(kc, df, dq[m]);
+                    if constexpr (MEND) pk[m] = mma(kc, pf, pk[m]);
+                }
             }
         }
     };
+    auto tile = [&](int t, const unsigned char* kt, const unsigned char* vt, auto next) {
+        if (t * KT + KT <= n) tile_of(std::true_type{}, t, kt, vt, next);
+        else tile_of(std::false_type{}, t, kt, vt, next);
+    };
     for (int t = t0; t < t1; t += 2) {
-        __syncthreads();
-        if (t + 1 < t1) issue(t + 1, buf1);
-        tile(t, buf0[0], buf0[1]);
+        tile_barrier();
+        tile(t, buf0[0], buf0[1], [&] { if (t + 1 < t1) issue(t + 1, buf1); });
         if (t + 1 < t1) {
-            __syncthreads();
-            if (t + 2 < t1) issue(t + 2, buf0);
-            tile(t + 1, buf1[0], buf1[1]);
+            tile_barrier();
+            tile(t + 1, buf1[0], buf1[1], [&] { if (t + 2 < t1) issue(t + 2, buf0); });
         }
+    }
+    if constexpr (MEND) e = halves_sum(e);
+    if (split == 0 && hh == 0) {
+        // (split: the launch that joins the sums adds the others' share to D; rows behind the last one have no share in anything)
+        float* rs = f.rows + ((int64_t)bh * f.nrb * 4 + rb * 4 + wave) * RSB + lane;
+        rs[0] = off;
+        rs[32] = fac;
+        rs[64] = f.nsq > 1 ? D : D + e;
     }
     if (!row_ok) return;
     if (f.nsq > 1) {
-        float* po = f.part_q + (((int64_t)split * p.B * p.Hkv + bh) * p.R + r) * HDP;
+        const int64_t row = ((int64_t)split * p.B * p.Hkv + bh) * p.R + r;
+        float* po = f.part_q + row * HDP * (MEND ? 2 : 1);
 #pragma unroll
         for (int m = 0; m < DM; ++m)
 #pragma unroll
-            for (int a = 0; a < 4; ++a) *(f32x4*)(po + 32 * m + 8 * a + 4 * hh) = (f32x4){dq[m][4 * a], dq[m][4 * a + 1], dq[m][4 * a + 2], dq[m][4 * a + 3]};
+            for (int a = 0; a < 4; ++a) {
+                const int d = 32 * m + 8 * a + 4 * hh;
+                *(f32x4*)(po + d) = (f32x4){dq[m][4 * a], dq[m][4 * a + 1], dq[m][4 * a + 2], dq[m][4 * a + 3]};
+                if constexpr (MEND) *(f32x4*)(po + HDP + d) = (f32x4){pk[m][4 * a], pk[m][4 * a + 1], pk[m][4 * a + 2], pk[m][4 * a + 3]};
+            }
+        if (MEND && hh == 0) f.part_e[row] = e;
         return;
     }
     T* out = (T*)f.dq + b * f.sdq.b + l * f.sdq.l + h * f.sdq.h;
@@ -160,7 +206,14 @@ __global__ __launch_bounds__(256, (HDP <= 64 && sizeof(T) == 2) ? 2 : 1) void cr
 #pragma unroll
         for (int a = 0; a < 4; ++a) {
             const int d = 32 * m + 8 * a + 4 * hh;
-            if (d < p.hd) store4(out + d, dq[m][4 * a] * p.scale, dq[m][4 * a + 1] * p.scale, dq[m][4 * a + 2] * p.scale, dq[m][4 * a + 3] * p.scale);
+            float v[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                v[c] = dq[m][4 * a + c];
+                if constexpr (MEND) v[c] = fmaf(-e, pk[m][4 * a + c], v[c]);
+                v[c] *= p.scale;
+            }
+            if (d < p.hd) store4(out + d, v[0], v[1], v[2], v[3]);
         }
 }
 
@@ -203,27 +256,44 @@ __global__ __launch_bounds__(256, (HDP <= 64 && sizeof(T) == 2) ? 2 : 1) void cr
         int t0, t1;
         split_range((p.R + QT - 1) / QT, split, f.nsk, t0, t1);
         const float* rows = f.rows + (int64_t)bh * f.nrb * 4 * RSB;
+        const unsigned char* qbase = (const unsigned char*)row_ptr<T>(p.q, p.sq, b, 0, 0);
+        const unsigned char* dobase = (const unsigned char*)row_ptr<T>(p.dout, p.sdo, b, 0, 0);
+        using FL = typename TL::template Fill<QT, 4>;
+        // (rows behind the last one: that one again - their P is 0)
         auto issue = [&](int t, unsigned char* dst) {
-            auto src = [&](const void* base, const Strides& s, int row) -> const unsigned char* {
-                const int r = t * QT + row;
-                if (r >= p.R) return nullptr;
+            int64_t oq[FL::FILLS], od[FL::FILLS];
+#pragma unroll
+            for (int i = 0; i < FL::FILLS; ++i) {
                 int l, h;
-                row_of(p, hk, r, l, h);
-                return (const unsigned char*)row_ptr<T>(base, s, b, l, h);
-            };
-            TL::template fill<QT, 4>(dst, wave, lane, hdb, [&](int row) { return src(p.q, p.sq, row); });
-            TL::template fill<QT, 4>(dst + TB, wave, lane, hdb, [&](int row) { return src(p.dout, p.sdo, row); });
+                row_of(p, hk, min(t * QT + FL::row_of_fill(i, wave, lane), p.R - 1), l, h);
+                oq[i] = (l * p.sq.l + h * p.sq.h) * (int)sizeof(T);
+                od[i] = (l * p.sdo.l + h * p.sdo.h) * (int)sizeof(T);
+            }
+            FL::run(dst, wave, lane, hdb, [&](int i) { return qbase + oq[i]; });
+            FL::run(dst + TB, wave, lane, hdb, [&](int i) { return dobase + od[i]; });
             // the row values: 512 bytes a block of 32 rows (they exist up to the next multiple of 128 rows)
             if (wave == 0 && lane < QT)
                 __builtin_amdgcn_global_load_lds((gbl_ptr_t)(rows + (int64_t)t * (QT / 32) * RSB + 4 * lane), (lds_ptr_t)(dst + 2 * TB), 16, 0, 0);
         };
         const float c2 = p.scale * LOG2E;
         const float* bcol = BIAS && attended ? p.bias + key : nullptr;
-        auto tile = [&](int t, const unsigned char* base) {
+        auto tile = [&](int t, const unsigned char* base, auto next) {
             const unsigned char *qt = base, *dot = base + TB;
 #pragma unroll
             for (int qb = 0; qb < QT / 32; ++qb) {
                 const float* rs = (const float*)(base + 2 * TB) + qb * RSB;
+                float bias[16];
+                if constexpr (BIAS) {
+                    const int r0 = t * QT + 32 * qb;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int r = r0 + acc_row(i, hh);
+                        int l, h;
+                        row_of(p, hk, min(r, p.R - 1), l, h);
+                        bias[i] = bcol != nullptr && r < p.R ? bcol[h * p.bias_h + l * p.bias_l] : 0.f;
+                    }
+                }
+                if (qb == 0) next();
                 f32x16 s = zero16(), dp = zero16();
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
@@ -238,16 +308,7 @@ __global__ __launch_bounds__(256, (HDP <= 64 && sizeof(T) == 2) ? 2 : 1) void cr
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int i = 4 * a + e;
-                        if constexpr (BIAS) {
-                            const int r = t * QT + 32 * qb + acc_row(i, hh);
-                            float bv = 0.f;
-                            if (r < p.R && bcol != nullptr) {
-                                int l, h;
-                                row_of(p, hk, r, l, h);
-                                bv = bcol[h * p.bias_h + l * p.bias_l];
-                            }
-                            s[i] = fmaf(s[i], p.scale, bv);
-                        }
+                        if constexpr (BIAS) s[i] = fmaf(s[i], p.scale, bias[i]);
                         const float pr = prob<BIAS>(s[i], c2, off[e], fac[e]);
                         s[i] = pr;
                         dp[i] = pr * (dp[i] - D[e]);
@@ -266,13 +327,11 @@ __global__ __launch_bounds__(256, (HDP <= 64 && sizeof(T) == 2) ? 2 : 1) void cr
         };
         if (t0 < t1) issue(t0, buf0);
         for (int t = t0; t < t1; t += 2) {
-            __syncthreads();
-            if (t + 1 < t1) issue(t + 1, buf1);
-            tile(t, buf0);
+            tile_barrier();
+            tile(t, buf0, [&] { if (t + 1 < t1) issue(t + 1, buf1); });
             if (t + 1 < t1) {
-                __syncthreads();
-                if (t + 2 < t1) issue(t + 2, buf0);
-                tile(t + 1, buf1);
+                tile_barrier();
+                tile(t + 1, buf1, [&] { if (t + 2 < t1) issue(t + 2, buf0); });
             }
         }
     }
@@ -323,7 +382,21 @@ __global__ __launch_bounds__(256) void cross_bwd_sum_kernel(const Bwd f) {
     const bool second = KEYS && blockIdx.y == 1;
     const float* part = KEYS ? (second ? f.part_v : f.part_k) : f.part_q;
     float a0 = 0.f, a1 = 0.f, a2 = 0.f, a3 = 0.f;
-    if (!KEYS || r < key_count(p, b)) {
+    if constexpr (!KEYS && sizeof(T) == 2) {
+        float e = 0.f, k0 = 0.f, k1 = 0.f, k2 = 0.f, k3 = 0.f;
+        for (int s = 0; s < ns; ++s) {
+            const float* po = part + (s * rows + g) * 2 * HDP + d;
+            const f32x4 v = *(const f32x4*)po, k = *(const f32x4*)(po + HDP);
+            a0 += v[0]; a1 += v[1]; a2 += v[2]; a3 += v[3];
+            k0 += k[0]; k1 += k[1]; k2 += k[2]; k3 += k[3];
+            e += f.part_e[s * rows + g];
+        }
+        a0 = fmaf(-e, k0, a0) * p.scale;
+        a1 = fmaf(-e, k1, a1) * p.scale;
+        a2 = fmaf(-e, k2, a2) * p.scale;
+        a3 = fmaf(-e, k3, a3) * p.scale;
+        if (d == 0) f.rows[((int64_t)bh * f.nrb * 4 + (r >> 5)) * RSB + 64 + (r & 31)] += e;
+    } else if (!KEYS || r < key_count(p, b)) {
         for (int s = 0; s < ns; ++s) {
             const f32x4 v = *(const f32x4*)(part + (s * rows + g) * HDP + d);
             a0 += v[0]; a1 += v[1]; a2 += v[2]; a3 += v[3];
@@ -344,19 +417,22 @@ __global__ __launch_bounds__(256) void cross_bwd_sum_kernel(const Bwd f) {
 }
 
 // dbias[h, i, j] = sum_b dS: grid (key tiles of 64, query blocks of 128, heads); keys are taken where they stand (the lists of attended keys
-// differ from entry to entry), with the key as lane column so that rows of bias and dbias are read and written in whole lines
+// differ from entry to entry), with the key as lane column so that rows of bias and dbias are read and written in whole lines.  While one
+// batch entry is worked on, the next one's K and V tiles, query rows and row values are on their way.
 template <typename T, int HDP>
-__global__ __launch_bounds__(256, 1) void cross_bwd_bias_kernel(const Bwd f) {
+__global__ __launch_bounds__(256, (HDP <= 64 && sizeof(T) == 2) ? 2 : 1) void cross_bwd_bias_kernel(const Bwd f) {
     using TL = Tile<T, HDP>;
     constexpr int KT = 64, TB = KT * TL::ROWB, KS = HDP / 16;
-    __shared__ __attribute__((aligned(16))) unsigned char buf[2][TB];
+    __shared__ __attribute__((aligned(16))) unsigned char buf0[2][TB];
+    __shared__ __attribute__((aligned(16))) unsigned char buf1[2][TB];
+    __shared__ __attribute__((aligned(16))) float rowv[4][3][32];
     const Prob& p = f.p;
     const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int j0 = blockIdx.x * KT, h = blockIdx.z, hk = h / p.grp, r0 = (h - hk * p.grp) * p.Lq;
     const int i0 = blockIdx.y * 128 + wave * 32;                    // this wave's query tokens
     const int hdb = p.hd * (int)sizeof(T);
-    const int l = min(i0 + (lane & 31), p.Lq - 1);
+    const int l = min(i0 + (lane & 31), p.Lq - 1), r = r0 + l;
     f32x16 acc[2] = {zero16(), zero16()};
     float bias[2][16];
 #pragma unroll
@@ -366,46 +442,76 @@ __global__ __launch_bounds__(256, 1) void cross_bwd_bias_kernel(const Bwd f) {
             const int li = min(i0 + acc_row(i, hh), p.Lq - 1), j = min(j0 + 32 * kb + (lane & 31), p.Lk - 1);
             bias[kb][i] = p.bias[h * p.bias_h + li * p.bias_l + j];
         }
-    for (int b = 0; b < p.B; ++b) {
-        const int len = f.kv_len == nullptr ? p.Lk : min(max(f.kv_len[b], 0), p.Lk);
-        if (j0 >= len) continue;                                    // (the same for the whole workgroup)
-        const unsigned char* kbase = (const unsigned char*)row_ptr<T>(p.k, p.sk, b, 0, hk);
-        const unsigned char* vbase = (const unsigned char*)row_ptr<T>(p.v, p.sv, b, 0, hk);
-        __syncthreads();
-        TL::template fill<KT, 4>(buf[0], wave, lane, hdb, [&](int row) { return kbase + min(j0 + row, len - 1) * p.sk.l * (int)sizeof(T); });
-        TL::template fill<KT, 4>(buf[1], wave, lane, hdb, [&](int row) { return vbase + min(j0 + row, len - 1) * p.sv.l * (int)sizeof(T); });
-        frag_t<T> qf[KS], dof[KS];
+    auto length = [&](int b) { return f.kv_len == nullptr ? p.Lk : min(max(f.kv_len[b], 0), p.Lk); };
+    // the next batch entry from b with keys in this tile (the same for the whole workgroup)
+    auto entry = [&](int b) {
+        while (b < p.B && j0 >= length(b)) ++b;
+        return b;
+    };
+    frag_t<T> qf[KS], dof[KS];
+    float off = 0.f, fac = 0.f, D = 0.f;
+    bool on[2];
+    auto fetch = [&](int b, unsigned char (&dst)[2][TB]) {
+        const int len = length(b);
         const T* qrow = row_ptr<T>(p.q, p.sq, b, l, h);
         const T* dorow = row_ptr<T>(p.dout, p.sdo, b, l, h);
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) { qf[ks] = load_frag<T>(qrow, ks, hh, p.hd); dof[ks] = load_frag<T>(dorow, ks, hh, p.hd); }
-        float off[16], fac[16], D[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int r = r0 + min(i0 + acc_row(i, hh), p.Lq - 1);
-            const float* rs = f.rows + (((int64_t)b * p.Hkv + hk) * f.nrb * 4 + (r >> 5)) * RSB + (r & 31);
-            off[i] = rs[0];
-            fac[i] = rs[32];
-            D[i] = rs[64];
-        }
-        __syncthreads();
+        const float* rs = f.rows + (((int64_t)b * p.Hkv + hk) * f.nrb * 4 + (r >> 5)) * RSB + (r & 31);
+        off = rs[0];
+        fac = rs[32];
+        D = rs[64];
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
             const int j = j0 + 32 * kb + (lane & 31);
-            const bool on = j < len && (f.mask == nullptr || f.mask[(int64_t)b * p.Lk + j] != 0);
+            on[kb] = j < len && (f.mask == nullptr || f.mask[(int64_t)b * p.Lk + j] != 0);
+        }
+        const unsigned char* kbase = (const unsigned char*)row_ptr<T>(p.k, p.sk, b, 0, hk);
+        const unsigned char* vbase = (const unsigned char*)row_ptr<T>(p.v, p.sv, b, 0, hk);
+        using FL = typename TL::template Fill<KT, 4>;
+        FL::run(dst[0], wave, lane, hdb, [&](int i) { return kbase + min(j0 + FL::row_of_fill(i, wave, lane), len - 1) * p.sk.l * (int)sizeof(T); });
+        FL::run(dst[1], wave, lane, hdb, [&](int i) { return vbase + min(j0 + FL::row_of_fill(i, wave, lane), len - 1) * p.sv.l * (int)sizeof(T); });
+    };
+    // one entry: its tiles are in cur; returns the entry whose fetch into the other buffer it started
+    auto work = [&](int b, unsigned char (&cur)[2][TB], unsigned char (&other)[2][TB]) {
+        rowv[wave][0][lane & 31] = off;                             // (both half-waves hold the same rows)
+        rowv[wave][1][lane & 31] = fac;
+        rowv[wave][2][lane & 31] = D;
+        frag_t<T> q[KS], d[KS];
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) { q[ks] = qf[ks]; d[ks] = dof[ks]; }
+        const bool on0 = on[0], on1 = on[1];
+        tile_barrier();
+        const int nb = entry(b + 1);
+        if (nb < p.B) fetch(nb, other);
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
             f32x16 s = zero16(), dp = zero16();
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                s = mma(qf[ks], TL::rows(buf[0], 32 * kb, ks, lane), s);
-                dp = mma(dof[ks], TL::rows(buf[1], 32 * kb, ks, lane), dp);
+                s = mma(q[ks], TL::rows(cur[0], 32 * kb, ks, lane), s);
+                dp = mma(d[ks], TL::rows(cur[1], 32 * kb, ks, lane), dp);
             }
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                // (a row that is not attended may hold anything: its values stay in this lane's column and are not used)
-                const float ds = prob<true>(fmaf(s[i], p.scale, bias[kb][i]), 0.f, off[i], fac[i]) * (dp[i] - D[i]);
-                acc[kb][i] += on ? ds : 0.f;
+            for (int a = 0; a < 4; ++a) {
+                const f32x4 o4 = *(const f32x4*)&rowv[wave][0][8 * a + 4 * hh], f4 = *(const f32x4*)&rowv[wave][1][8 * a + 4 * hh],
+                            d4 = *(const f32x4*)&rowv[wave][2][8 * a + 4 * hh];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int i = 4 * a + e;
+                    // (a row that is not attended may hold anything: its values stay in this lane's column and are not used)
+                    const float ds = prob<true>(fmaf(s[i], p.scale, bias[kb][i]), 0.f, o4[e], f4[e]) * (dp[i] - d4[e]);
+                    acc[kb][i] += (kb == 0 ? on0 : on1) ? ds : 0.f;
+                }
             }
         }
+        return nb;
+    };
+    int b = entry(0);
+    if (b < p.B) fetch(b, buf0);
+    while (b < p.B) {
+        b = work(b, buf0, buf1);
+        if (b < p.B) b = work(b, buf1, buf0);
     }
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
@@ -416,7 +522,7 @@ __global__ __launch_bounds__(256, 1) void cross_bwd_bias_kernel(const Bwd f) {
         }
 }
 
-struct BwdPlan { int hdp, nrb, nsq, nkb, nsk; int64_t rows_bytes, q_bytes, k_bytes; };
+struct BwdPlan { int hdp, nrb, nsq, nkb, nsk; int64_t rows_bytes, q_bytes, e_bytes, k_bytes; };
 int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
 
 int splits(int64_t blocks, int64_t most) {
@@ -435,7 +541,8 @@ BwdPlan plan_bwd(const MarsCrossAttn* a) {
     pl.nsq = splits(nbh * pl.nrb, ((int64_t)a->Lk + 127) / 128);
     pl.nsk = splits(nbh * pl.nkb, (R + 127) / 128);
     pl.rows_bytes = align256(nbh * pl.nrb * 4 * RSB * 4);
-    pl.q_bytes = pl.nsq > 1 ? align256((int64_t)pl.nsq * nbh * R * pl.hdp * 4) : 0;
+    pl.q_bytes = pl.nsq > 1 ? align256((int64_t)pl.nsq * nbh * R * pl.hdp * 4 * (a->dtype == 1 ? 2 : 1)) : 0;
+    pl.e_bytes = pl.nsq > 1 && a->dtype == 1 ? align256((int64_t)pl.nsq * nbh * R * 4) : 0;
     pl.k_bytes = pl.nsk > 1 ? align256((int64_t)pl.nsk * nbh * a->Lk * pl.hdp * 4) : 0;
     return pl;
 }
@@ -481,7 +588,7 @@ template <typename T> int launch_bwd_hd(const Bwd& f, int hdp, hipStream_t s) {
 
 int64_t bwd_ws_bytes(const MarsCrossAttn* a) {
     const BwdPlan pl = plan_bwd(a);
-    return pl.rows_bytes + pl.q_bytes + 2 * pl.k_bytes;
+    return pl.rows_bytes + pl.q_bytes + pl.e_bytes + 2 * pl.k_bytes;
 }
 
 }  // namespace xattn
@@ -500,8 +607,9 @@ extern "C" int marship_cross_attn_bwd(const MarsCrossAttn* a, void* stream) {
     char* w = (char*)a->ws + key_ws_bytes(a);
     f.rows = (float*)w;
     f.part_q = (float*)(w + pl.rows_bytes);
-    f.part_k = (float*)(w + pl.rows_bytes + pl.q_bytes);
-    f.part_v = (float*)(w + pl.rows_bytes + pl.q_bytes + pl.k_bytes);
+    f.part_e = (float*)(w + pl.rows_bytes + pl.q_bytes);
+    f.part_k = (float*)(w + pl.rows_bytes + pl.q_bytes + pl.e_bytes);
+    f.part_v = (float*)(w + pl.rows_bytes + pl.q_bytes + pl.e_bytes + pl.k_bytes);
     f.dq = a->dq; f.dk = a->dk; f.dv = a->dv;
     f.sdq = Strides{a->dq_s[0], a->dq_s[1], a->dq_s[2]};
     f.sdk = Strides{a->dk_s[0], a->dk_s[1], a->dk_s[2]};
