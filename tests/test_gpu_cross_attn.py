@@ -127,11 +127,20 @@ def reference(c):
             D = (dO * O).sum(1, keepdim=True)
             dS = P * (dP - D)
             mdP = dO.abs() @ V.abs().t()
-            tD = (dO.abs() * tO).sum(1, keepdim=True) + hd * U32 * (dO * O).abs().sum(1, keepdim=True)
-            tS = P * ((dP - D).abs() * (r + 4 * U32) + tD + (hd + 2) * U32 * mdP)
+            e0 = (dO.abs() * tO).sum(1, keepdim=True)                               # D' = dO . (rounded O) against D
+            t1 = P * (dP - D).abs() * (r + 4 * U32) + P * mdP * (hd + 2) * U32      # of dS, but for D
+            tE = (t1 + P * ((dP - D).abs() + e0) * (r + n * U32)).sum(1, keepdim=True)
+            # bf16: D = D' + sum dS' (the probabilities add up to 1 within r); f32: D = D'
+            tD = tE + (D.abs() + e0) * (r + 2 * U32) if u else e0 + hd * U32 * (dO * O).abs().sum(1, keepdim=True)
+            tS = t1 + P * tD
             tSr = tS + u * dS.abs() * 1.01                                          # rounded for the matrix instruction
+            PK = P @ K.abs()
             res["dq"][b, :, h] = dS @ K * c["scale"]
-            tol["dq"][b, :, h] = c["scale"] * ((tSr + n * U32 * dS.abs()) @ K.abs()) + ro * res["dq"][b, :, h].abs() + 1e-30
+            if u:       # sum dS' K - e sum P K: dS' and P rounded, e = D' - D of the size e0
+                tq = (t1 + u * (dS.abs() + P * e0) * 1.01 + n * U32 * (dS.abs() + P * e0)) @ K.abs() + (e0 * (u + r + n * U32) + tD) * PK
+            else:
+                tq = (tS + n * U32 * dS.abs()) @ K.abs()
+            tol["dq"][b, :, h] = c["scale"] * tq + ro * res["dq"][b, :, h].abs() + 1e-30
             res["dk"][b, keys, j] += dS.t() @ Q * c["scale"]
             tol["dk"][b, keys, j] += c["scale"] * ((tSr + H * Lq * U32 * dS.abs()).t() @ Q.abs())
             res["dv"][b, keys, j] += P.t() @ dO
