@@ -56,6 +56,9 @@ template <typename T> __device__ __forceinline__ frag_t<T> pack_step(const f32x1
 // row of accumulator register i in a 32-row block
 __device__ __forceinline__ int acc_row(int i, int hh) { return 8 * (i >> 2) + 4 * hh + (i & 3); }
 
+// the larger of two values, NaN if one is (v_maximum3_f32; fmaxf would first quieten each operand with an instruction of its own)
+__device__ __forceinline__ float vmax(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
 // x of this lane combined with x of the same column in the other half-wave
 __device__ __forceinline__ float halves_sum(float x) {
     const unsigned u = __builtin_bit_cast(unsigned, x);
@@ -65,7 +68,7 @@ __device__ __forceinline__ float halves_sum(float x) {
 __device__ __forceinline__ float halves_max(float x) {
     const unsigned u = __builtin_bit_cast(unsigned, x);
     const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-    return fmaxf(__builtin_bit_cast(float, (unsigned)r[0]), __builtin_bit_cast(float, (unsigned)r[1]));
+    return vmax(__builtin_bit_cast(float, (unsigned)r[0]), __builtin_bit_cast(float, (unsigned)r[1]));
 }
 
 // ---- LDS tiles: rows of HDP elements in 16-byte chunks, filled by LDS-DMA.  Chunk c of row r sits at slot

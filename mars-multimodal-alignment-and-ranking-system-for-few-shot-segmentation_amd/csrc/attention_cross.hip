@@ -164,8 +164,8 @@ __global__ __launch_bounds__(256, (FwdCfg<T, HDP, FEW>::WPE)) void cross_fwd_ker
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb][i]);
-        const float mnew = fmaxf(mrun, halves_max(mx));
+            for (int i = 0; i < 16; ++i) mx = vmax(mx, s[kb][i]);
+        const float mnew = vmax(mrun, halves_max(mx));
         // (a bias of -inf on every key so far: nothing to scale, and the exponentials must come out as zeros)
         const float mref = BIAS && mnew == -INFINITY ? 0.f : mnew;
         const float unit = BIAS ? LOG2E : c2;
@@ -197,54 +197,81 @@ __global__ __launch_bounds__(256, (FwdCfg<T, HDP, FEW>::WPE)) void cross_fwd_ker
                 for (int m = 0; m < DM; ++m) o[m] = mma(TL::cols(vt, 32 * kb + 16 * u, m, lane), pf, o[m]);
             }
     };
-    auto tile = [&](int t, const unsigned char* kt, const unsigned char* vt, auto next) {
-        if (t * KT + KT <= n) tile_of(std::true_type{}, t, kt, vt, next);
-        else tile_of(std::false_type{}, t, kt, vt, next);
-    };
+    // whole tiles in the loops, the ragged one behind them: both forms inside one loop would make the compiler carry the accumulators
+    // through the join in a second set of registers
+    const int tw = min(t1, n / KT);
+    constexpr std::true_type whole{};
+    constexpr std::false_type ragged{};
     auto nothing = [] {};
 
     if constexpr (!FEW) {
         look_up(t0);
         if (t0 < t1) issue(t0, buf0[0][0]);
+        int t = t0;
         if constexpr (Cfg::BUFS == 2) {
-            for (int t = t0; t < t1; t += 2) {
+            bool odd = false;
+            while (t < tw) {
                 tile_barrier();
-                tile(t, buf0[0][0], buf0[0][1], [&] { if (t + 1 < t1) issue(t + 1, buf1[0][0]); });
-                if (t + 1 < t1) {
-                    tile_barrier();
-                    tile(t + 1, buf1[0][0], buf1[0][1], [&] { if (t + 2 < t1) issue(t + 2, buf0[0][0]); });
-                }
+                tile_of(whole, t, buf0[0][0], buf0[0][1], [&] { if (t + 1 < t1) issue(t + 1, buf1[0][0]); });
+                odd = true;
+                if (++t >= tw) break;
+                tile_barrier();
+                tile_of(whole, t, buf1[0][0], buf1[0][1], [&] { if (t + 1 < t1) issue(t + 1, buf0[0][0]); });
+                odd = false;
+                ++t;
+            }
+            if (t < t1) {
+                tile_barrier();
+                const unsigned char* at = odd ? buf1[0][0] : buf0[0][0];
+                tile_of(ragged, t, at, at + TB, nothing);
             }
         } else {
-            for (int t = t0; t < t1; ++t) {
+            for (; t < tw; ++t) {
                 tile_barrier();
-                tile(t, buf0[0][0], buf0[0][1], nothing);
+                tile_of(whole, t, buf0[0][0], buf0[0][1], nothing);
                 tile_barrier();
                 if (t + 1 < t1) issue(t + 1, buf0[0][0]);
+            }
+            if (t < t1) {
+                tile_barrier();
+                tile_of(ragged, t, buf0[0][0], buf0[0][1], nothing);
             }
         }
     } else {
         unsigned char* my0 = buf0[cw][0];
         unsigned char* my1 = Cfg::BUFS == 2 ? buf1[Cfg::BUFS == 2 ? cw : 0][0] : my0;
-        // waves without a tile skip the loops; a wave's own buffers need its own waits only
-        const int first = t0 + wave;
-        look_up(first);
-        if (first < t1) issue(first, my0);
+        // a wave's own buffers need its own waits only
+        int t = t0 + wave;
+        look_up(t);
+        if (t < t1) issue(t, my0);
         if constexpr (Cfg::BUFS == 2) {
-            for (int t = first; t < t1; t += 8) {
+            bool odd = false;
+            while (t < tw) {
                 __builtin_amdgcn_s_waitcnt(0);
-                tile(t, my0, my0 + TB, [&] { if (t + 4 < t1) issue(t + 4, my1); });
-                if (t + 4 < t1) {
-                    __builtin_amdgcn_s_waitcnt(0);
-                    tile(t + 4, my1, my1 + TB, [&] { if (t + 8 < t1) issue(t + 8, my0); });
-                }
+                tile_of(whole, t, my0, my0 + TB, [&] { if (t + 4 < t1) issue(t + 4, my1); });
+                odd = true;
+                t += 4;
+                if (t >= tw) break;
+                __builtin_amdgcn_s_waitcnt(0);
+                tile_of(whole, t, my1, my1 + TB, [&] { if (t + 4 < t1) issue(t + 4, my0); });
+                odd = false;
+                t += 4;
+            }
+            if (t < t1) {
+                __builtin_amdgcn_s_waitcnt(0);
+                const unsigned char* at = odd ? my1 : my0;
+                tile_of(ragged, t, at, at + TB, nothing);
             }
         } else {
-            for (int t = first; t < t1; t += 4) {
+            for (; t < tw; t += 4) {
                 __builtin_amdgcn_s_waitcnt(0);
-                tile(t, my0, my0 + TB, nothing);
+                tile_of(whole, t, my0, my0 + TB, nothing);
                 __builtin_amdgcn_s_waitcnt(0);
                 if (t + 4 < t1) issue(t + 4, my0);
+            }
+            if (t < t1) {
+                __builtin_amdgcn_s_waitcnt(0);
+                tile_of(ragged, t, my0, my0 + TB, nothing);
             }
         }
     }
@@ -259,7 +286,7 @@ __global__ __launch_bounds__(256, (FwdCfg<T, HDP, FEW>::WPE)) void cross_fwd_ker
         if (hh == 0) { xs[(wave * 32 + lane) * 2] = mrun; xs[(wave * 32 + lane) * 2 + 1] = lsum; }
         __syncthreads();
         float mall = -INFINITY, lall = 0.f;
-        for (int w = 0; w < 4; ++w) mall = fmaxf(mall, xs[(w * 32 + (lane & 31)) * 2]);
+        for (int w = 0; w < 4; ++w) mall = vmax(mall, xs[(w * 32 + (lane & 31)) * 2]);
         const float mref = mall == -INFINITY ? 0.f : mall;
         const float unit = BIAS ? LOG2E : c2;
         for (int w = 0; w < 4; ++w) {
@@ -325,7 +352,7 @@ __global__ __launch_bounds__(256) void cross_join_kernel(const Fwd f) {
     const int d = 4 * (threadIdx.x % LR);
     if (threadIdx.x >= 256 / LR * LR || g >= rows) return;
     float m = -INFINITY;
-    for (int s = 0; s < f.ns; ++s) m = fmaxf(m, f.part_s[(s * rows + g) * 2]);
+    for (int s = 0; s < f.ns; ++s) m = vmax(m, f.part_s[(s * rows + g) * 2]);
     const float mref = m == -INFINITY ? 0.f : m;
     float l = 0.f, a0 = 0.f, a1 = 0.f, a2 = 0.f, a3 = 0.f;
     for (int s = 0; s < f.ns; ++s) {

@@ -29,6 +29,7 @@ namespace {
 // and factor = 1 / sum: where the mask is the type's lowest value the sum's logarithm would be lost in the maximum.
 // Rows that do not exist or have no key: P = 0.
 constexpr int RSB = 128;
+constexpr int QW = 96, KW = 96;
 
 struct Bwd {
     Prob p;
@@ -50,7 +51,7 @@ template <bool BIAS> __device__ __forceinline__ float prob(float s, float c2, fl
 }
 
 template <typename T, int HDP, bool BIAS>
-__global__ __launch_bounds__(256, (HDP <= 64 && sizeof(T) == 2) ? 2 : 1) void cross_bwd_q_kernel(const Bwd f) {
+__global__ __launch_bounds__(256, (HDP <= QW && sizeof(T) == 2) ? 2 : 1) void cross_bwd_q_kernel(const Bwd f) {
     using TL = Tile<T, HDP>;
     constexpr int KT = (HDP > 64 && sizeof(T) == 4) ? 32 : 64, TB = KT * TL::ROWB, KB = KT / 32, KS = HDP / 16, DM = HDP / 32;
     __shared__ __attribute__((aligned(16))) unsigned char buf0[2][TB];
@@ -163,19 +164,27 @@ __global__ __launch_bounds__(256, (HDP <= 64 && sizeof(T) == 2) ? 2 : 1) void cr
                     if constexpr (MEND) pk[m] = mma(kc, pf, pk[m]);
                 }
             }
+            if constexpr (HDP > 64) __builtin_amdgcn_sched_barrier(0);  // (two blocks in flight would not fit the registers)
         }
     };
-    auto tile = [&](int t, const unsigned char* kt, const unsigned char* vt, auto next) {
-        if (t * KT + KT <= n) tile_of(std::true_type{}, t, kt, vt, next);
-        else tile_of(std::false_type{}, t, kt, vt, next);
-    };
-    for (int t = t0; t < t1; t += 2) {
+    // (whole tiles in the loop, the ragged one behind it: as in the forward pass)
+    const int tw = min(t1, n / KT);
+    int t = t0;
+    bool odd = false;
+    while (t < tw) {
         tile_barrier();
-        tile(t, buf0[0], buf0[1], [&] { if (t + 1 < t1) issue(t + 1, buf1); });
-        if (t + 1 < t1) {
-            tile_barrier();
-            tile(t + 1, buf1[0], buf1[1], [&] { if (t + 2 < t1) issue(t + 2, buf0); });
-        }
+        tile_of(std::true_type{}, t, buf0[0], buf0[1], [&] { if (t + 1 < t1) issue(t + 1, buf1); });
+        odd = true;
+        if (++t >= tw) break;
+        tile_barrier();
+        tile_of(std::true_type{}, t, buf1[0], buf1[1], [&] { if (t + 1 < t1) issue(t + 1, buf0); });
+        odd = false;
+        ++t;
+    }
+    if (t < t1) {
+        tile_barrier();
+        const unsigned char* at = odd ? buf1[0] : buf0[0];
+        tile_of(std::false_type{}, t, at, at + TB, [] {});
     }
     if constexpr (MEND) e = halves_sum(e);
     if (split == 0 && hh == 0) {
@@ -223,7 +232,7 @@ template <typename T, int HDP> struct KeyCfg {
 };
 
 template <typename T, int HDP, bool BIAS>
-__global__ __launch_bounds__(256, (HDP <= 64 && sizeof(T) == 2) ? 2 : 1) void cross_bwd_kv_kernel(const Bwd f) {
+__global__ __launch_bounds__(256, (HDP <= KW && sizeof(T) == 2) ? 2 : 1) void cross_bwd_kv_kernel(const Bwd f) {
     using TL = Tile<T, HDP>;
     using Cfg = KeyCfg<T, HDP>;
     constexpr int QT = Cfg::QT, TB = Cfg::TB, KS = HDP / 16, DM = HDP / 32;
