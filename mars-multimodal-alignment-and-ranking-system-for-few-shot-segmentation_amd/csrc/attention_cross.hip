@@ -342,31 +342,58 @@ __global__ __launch_bounds__(256, (FwdCfg<T, HDP, FEW>::WPE)) void cross_fwd_ker
     }
 }
 
-// joins the splits: 64 / (HDP / 4) rows a wave, a lane owns four elements of a row
+// Joins the splits.  A lane owns four elements of a row, HDP / 4 lanes a row; where the splits outnumber it, 64 / (HDP / 4) lane groups of a wave take the splits
+// of one row in turn (each with its own running maximum) and meet in shuffles: the loads of a row are few trips to memory deep.
 template <typename T, int HDP>
 __global__ __launch_bounds__(256) void cross_join_kernel(const Fwd f) {
-    constexpr int LR = HDP / 4;
+    constexpr int LR = HDP / 4 == 24 ? 32 : HDP / 4, NG = 64 / LR;          // lanes a row (96: eight of 32 stay idle), groups a wave
     const Prob& p = f.p;
     const int64_t rows = (int64_t)p.B * p.Hkv * p.R;
-    const int64_t g = (int64_t)blockIdx.x * (256 / LR) + threadIdx.x / LR;
-    const int d = 4 * (threadIdx.x % LR);
-    if (threadIdx.x >= 256 / LR * LR || g >= rows) return;
-    float m = -INFINITY;
-    for (int s = 0; s < f.ns; ++s) m = vmax(m, f.part_s[(s * rows + g) * 2]);
-    const float mref = m == -INFINITY ? 0.f : m;
-    float l = 0.f, a0 = 0.f, a1 = 0.f, a2 = 0.f, a3 = 0.f;
-    for (int s = 0; s < f.ns; ++s) {
-        const float ls = f.part_s[(s * rows + g) * 2 + 1];
-        const float w = __builtin_amdgcn_exp2f((f.part_s[(s * rows + g) * 2] - mref) * LOG2E);
-        const f32x4 v = *(const f32x4*)(f.part_o + (s * rows + g) * HDP + d);
-        l = fmaf(ls, w, l);
-        a0 = fmaf(v[0], w, a0); a1 = fmaf(v[1], w, a1); a2 = fmaf(v[2], w, a2); a3 = fmaf(v[3], w, a3);
+    const int lane = threadIdx.x & 63, grp = lane / LR, d = 4 * (lane % LR);
+    const int64_t g = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (g >= rows) return;
+    const bool on = d < HDP;
+    float m = -INFINITY, l = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    auto add = [&](float mo, float lo, const f32x4& v) {
+        const float mn = vmax(m, mo), ref = mn == -INFINITY ? 0.f : mn;
+        const float wa = __builtin_amdgcn_exp2f((m - ref) * LOG2E), wb = __builtin_amdgcn_exp2f((mo - ref) * LOG2E);
+        l = l * wa + lo * wb;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] = acc[e] * wa + v[e] * wb;
+        m = mn;
+    };
+    constexpr int U = 4;
+    for (int s0 = grp; s0 < f.ns; s0 += NG * U) {
+        float ms[U], ls[U];
+        f32x4 v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int s = s0 + u * NG;
+            ms[u] = -INFINITY;
+            ls[u] = 0.f;
+            v[u] = (f32x4){0.f, 0.f, 0.f, 0.f};
+            if (s < f.ns) {
+                ms[u] = f.part_s[(s * rows + g) * 2];
+                ls[u] = f.part_s[(s * rows + g) * 2 + 1];
+                if (on) v[u] = *(const f32x4*)(f.part_o + (s * rows + g) * HDP + d);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) add(ms[u], ls[u], v[u]);
     }
+#pragma unroll
+    for (int o = LR; o < 64; o <<= 1) {
+        const float mo = __shfl_xor(m, o, 64), lo = __shfl_xor(l, o, 64);
+        const f32x4 v = {__shfl_xor(acc[0], o, 64), __shfl_xor(acc[1], o, 64), __shfl_xor(acc[2], o, 64), __shfl_xor(acc[3], o, 64)};
+        add(mo, lo, v);
+    }
+    if (grp != 0) return;
     const int bh = (int)(g / p.R), r = (int)(g - (int64_t)bh * p.R), b = bh / p.Hkv, hk = bh - b * p.Hkv;
     int tok, h;
     row_of(p, hk, r, tok, h);
     const float inv = l == 0.f ? 0.f : 1.0f / l;
-    if (d < p.hd) store4((T*)f.out + b * p.so.b + tok * p.so.l + h * p.so.h + d, a0 * inv, a1 * inv, a2 * inv, a3 * inv);
+    if (on && d < p.hd) store4((T*)f.out + b * p.so.b + tok * p.so.l + h * p.so.h + d, acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
     if (f.stat != nullptr && d == 0) {
         float* st = f.stat + (((int64_t)b * p.H + h) * p.Lq + tok) * 2;
         st[0] = m;
@@ -408,8 +435,9 @@ template <typename T, int HDP> int launch_fwd(const Fwd& f, bool few, hipStream_
     }
     MARS_LAUNCH_CHECK();
     if (f.ns > 1) {
-        const int64_t rows = (int64_t)f.p.B * f.p.Hkv * f.p.R, per = 256 / (HDP / 4);
-        hipLaunchKernelGGL((cross_join_kernel<T, HDP>), dim3((unsigned)((rows + per - 1) / per)), block, 0, s, f);
+        const int64_t rows = (int64_t)f.p.B * f.p.Hkv * f.p.R;
+        MARS_CHECK((rows + 3) / 4 * 256 < (1ll << 32), "cross_attn: more workgroups than a launch takes");
+        hipLaunchKernelGGL((cross_join_kernel<T, HDP>), dim3((unsigned)((rows + 3) / 4)), block, 0, s, f);
         MARS_LAUNCH_CHECK();
     }
     return 0;

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import bisect
 import ctypes
+import struct
 from typing import Optional
 
 import torch
@@ -1017,6 +1018,34 @@ def mask_embed(masks: torch.Tensor, G: int, params, eps: float, out: torch.Tenso
 
 
 # ---------------------------------------------------------------- a trained cross-attention block over patch features
+# The entry points below are called on small problems too (one new token, the prompt tokens of a mask), where checking and describing
+# the operands in Python is longer than the kernels.  So a call's checks and the argument block they end in are kept by LAYOUT - shapes, strides,
+# types, scalars; never by address - and a call with a known layout only fills in its pointers.
+_PLANS: dict = {}
+
+
+def _plan(key, build):
+    plan = _PLANS.get(key)
+    if plan is None:
+        plan = build()
+        if len(_PLANS) >= 1024:
+            _PLANS.clear()
+        _PLANS[key] = plan
+    return plan
+
+
+def _lay(t: Optional[torch.Tensor]):
+    return None if t is None else (t.shape, t.stride(), t.dtype)
+
+
+def _on_device(*ts):
+    """``_dev`` without its cost where everything is in order"""
+    cur = torch.cuda.current_device() if torch.cuda.is_initialized() else None
+    for t in ts:
+        if t is not None and t.get_device() != cur:
+            _dev(*ts)
+
+
 def _workspace(nbytes: int, device) -> Optional[torch.Tensor]:
     """A workspace of one call, from torch's caching allocator: ordered on the call's stream, and inside a captured graph's own
     pool, so that two calls, streams or graphs never share one."""
@@ -1031,30 +1060,28 @@ def _own_elements(t: torch.Tensor, what: str):
         end = st * (n - 1) + end
 
 
-def _not_an_input(outs, ins, what: str):
-    """No output starts where another operand does (a result written over an operand that is still being read)."""
-    taken = {t.data_ptr() for t in ins if t is not None}
-    for t in outs:
-        if t is not None:
-            _req(t.data_ptr() not in taken, f"{what}: an output lies on another operand")
-            taken.add(t.data_ptr())
-
-
 def _rows16(what: str, **views):
     for name, t in views.items():
         es = t.element_size()
         _req(t.dim() == 4, f"{what}: {name} must be [batch, tokens, heads, head dim]")
         _req(t.stride(3) == 1 or t.shape[3] == 1, f"{what}: {name}: the elements of a head must be contiguous")
-        _req(t.data_ptr() % 16 == 0 and all((t.stride(d) * es) % 16 == 0 for d in range(3) if t.shape[d] > 1),
-             f"{what}: {name}: rows must be 16-byte aligned")
+        _req(all((t.stride(d) * es) % 16 == 0 for d in range(3) if t.shape[d] > 1), f"{what}: {name}: rows must be 16-byte aligned")
 
 
 def _strides3(t: torch.Tensor):
     return (ctypes.c_int64 * 3)(*(t.stride(d) if t.shape[d] > 1 else 0 for d in range(3)))
 
 
-def _cross_args(what, q, k, v, out, stat, scale, kv_len, mask, bias) -> MarsCrossAttn:
-    _dev(q, k, v, out, stat, kv_len, mask, bias)
+def _strides2(t: torch.Tensor):
+    return (ctypes.c_int64 * 2)(*(t.stride(d) if t.shape[d] > 1 else 0 for d in range(2)))
+
+
+_PTRS8, _PTRS5, _PTRS2 = struct.Struct("8Q"), struct.Struct("5Q"), struct.Struct("2Q")
+_OFF_BWD, _OFF_WS = MarsCrossAttn.dout.offset, MarsCrossAttn.ws.offset
+
+
+def _cross_block(what, q, k, v, out, stat, scale, kv_len, mask, bias) -> MarsCrossAttn:
+    """checks of everything but addresses, and the argument block without its pointers"""
     _rows16(what, q=q, k=k, v=v, out=out)
     _req(q.dtype == k.dtype == v.dtype == out.dtype and q.dtype in (torch.float32, torch.bfloat16), f"{what}: one dtype, f32 or bf16")
     B, Lq, H, hd = q.shape
@@ -1063,26 +1090,28 @@ def _cross_args(what, q, k, v, out, stat, scale, kv_len, mask, bias) -> MarsCros
     _req(tuple(k.shape) == (B, Lk, Hkv, hd) and tuple(v.shape) == (B, Lk, Hkv, hd) and out.shape == q.shape, f"{what}: shape mismatch")
     _req(H % Hkv == 0, f"{what}: {H} query heads are no multiple of {Hkv} key heads")
     _req(hd <= 128 and (hd * q.element_size()) % 16 == 0, f"{what}: head dim {hd} (up to 128, a multiple of 16 bytes)")
+    _own_elements(out, what)
     a = MarsCrossAttn()
     if stat is not None:
         _req(stat.dtype == torch.float32 and stat.is_contiguous() and tuple(stat.shape) == (B, H, Lq, 2), f"{what}: stat must be contiguous f32 [B, H, Lq, 2]")
-        a.stat = stat.data_ptr()
     if kv_len is not None:
         _req(kv_len.dtype == torch.int32 and kv_len.is_contiguous() and tuple(kv_len.shape) == (B,), f"{what}: kv_len must be i32 [B]")
-        a.kv_len = kv_len.data_ptr()
     if mask is not None:
         _req(mask.dtype in (torch.uint8, torch.bool) and mask.is_contiguous() and tuple(mask.shape) == (B, Lk),
              f"{what}: mask must be contiguous u8 or bool [B, Lk]")
-        a.mask = mask.data_ptr()
+        a.mask = 1                                              # (the workspace depends on whether there is one)
     if bias is not None:
         _req(bias.dtype == torch.float32 and tuple(bias.shape) == (H, Lq, Lk) and (bias.stride(2) == 1 or Lk == 1), f"{what}: bias must be f32 [H, Lq, Lk]")
-        a.bias, a.bias_s = bias.data_ptr(), (ctypes.c_int64 * 2)(bias.stride(0), bias.stride(1))
+        a.bias_s = _strides2(bias)
     scale = hd ** -0.5 if scale is None else float(scale)
     _req(0.0 < scale < float("inf"), f"{what}: scale must be positive and finite")
-    a.q, a.k, a.v, a.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
     a.q_s, a.k_s, a.v_s, a.out_s = _strides3(q), _strides3(k), _strides3(v), _strides3(out)
     a.B, a.Lq, a.Lk, a.H, a.Hkv, a.hd, a.scale, a.dtype = B, Lq, Lk, H, Hkv, hd, scale, dt(q)
     return a
+
+
+def _addr(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def cross_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, *, stat: Optional[torch.Tensor] = None,
@@ -1094,15 +1123,25 @@ def cross_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Ten
     ``kv_len`` i32 [B]: keys at or behind it are not attended; ``mask`` u8 or bool [B, Lk]: only keys with a non-zero entry are; what K and V
     hold at the others is not read.  ``bias`` f32 [H, Lq, Lk], shared by the batch (-inf and the lowest float are allowed).  A row
     without a key gives zeros.  ``scale`` defaults to hd ** -0.5.  ``stat`` f32 [B, H, Lq, 2] receives what ``cross_attn_bwd`` needs."""
-    a = _cross_args("cross_attn", q, k, v, out, stat, scale, kv_len, mask, bias)
-    _own_elements(out, "cross_attn")
-    _not_an_input((out, stat), (q, k, v, kv_len, mask, bias), "cross_attn")
+    _on_device(q, k, v, out, stat, kv_len, mask, bias)
     lib = hip.lib()
-    nws = lib.marship_cross_attn_ws(ctypes.byref(a), 0)
-    ws = _workspace(nws, q.device)
-    if ws is not None:
-        a.ws, a.ws_bytes = ws.data_ptr(), nws
-    hip.check(lib.marship_cross_attn(ctypes.byref(a), stream()), "marship_cross_attn")
+
+    def build():
+        a = _cross_block("cross_attn", q, k, v, out, stat, scale, kv_len, mask, bias)
+        return bytes(a), lib.marship_cross_attn_ws(ctypes.byref(a), 0)
+
+    block, nws = _plan((1, scale, _lay(q), _lay(k), _lay(v), _lay(out), _lay(stat), _lay(kv_len), _lay(mask), _lay(bias)), build)
+    pq, pk, pv, po, ps = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _addr(stat)
+    _req((pq | pk | pv | po) % 16 == 0, "cross_attn: rows must be 16-byte aligned")
+    pb, pl, pm = _addr(bias), _addr(kv_len), _addr(mask)
+    ins = (pq, pk, pv, pb, pl, pm)
+    _req(po not in ins and (ps == 0 or ps not in ins) and po != ps, "cross_attn: an output lies on another operand")
+    buf = bytearray(block)
+    _PTRS8.pack_into(buf, 0, pq, pk, pv, po, ps, pb, pl, pm)
+    if nws:
+        ws = _workspace(nws, q.device)
+        _PTRS2.pack_into(buf, _OFF_WS, ws.data_ptr(), nws)
+    hip.check(lib.marship_cross_attn(ctypes.byref(MarsCrossAttn.from_buffer(buf)), stream()), "marship_cross_attn")
 
 
 def cross_attn_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, stat: torch.Tensor, dout: torch.Tensor,
@@ -1111,28 +1150,40 @@ def cross_attn_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch
     """Gradients of ``cross_attn`` from its operands, its ``out`` and ``stat`` and the gradient ``dout`` of ``out``: dq, dk, dv (zeros at keys that are
     not attended) and, where ``dbias`` f32 [H, Lq, Lk] is given, the bias's, summed over the batch.  The same ``scale``, ``kv_len``, ``mask`` and
     ``bias`` as in the forward call.  Sums have a fixed order: the same call gives the same bits."""
-    a = _cross_args("cross_attn_bwd", q, k, v, out, stat, scale, kv_len, mask, bias)
-    _req(stat is not None, "cross_attn_bwd: stat of the forward call is needed")
-    _dev(dout, dq, dk, dv, dbias)
-    _rows16("cross_attn_bwd", dout=dout, dq=dq, dk=dk, dv=dv)
-    _req(all(t.dtype == q.dtype for t in (dout, dq, dk, dv)), "cross_attn_bwd: one dtype, f32 or bf16")
-    _req(dout.shape == q.shape and dq.shape == q.shape and dk.shape == k.shape and dv.shape == v.shape, "cross_attn_bwd: shape mismatch")
-    if dbias is not None:
-        _req(bias is not None, "cross_attn_bwd: a gradient of a bias that is not there")
-        _req(dbias.dtype == torch.float32 and dbias.shape == bias.shape and (dbias.stride(2) == 1 or dbias.shape[2] == 1),
-             "cross_attn_bwd: dbias must be f32 [H, Lq, Lk]")
-        _own_elements(dbias, "cross_attn_bwd")
-        a.dbias, a.dbias_s = dbias.data_ptr(), (ctypes.c_int64 * 2)(dbias.stride(0), dbias.stride(1))
-    for t in (dq, dk, dv):
-        _own_elements(t, "cross_attn_bwd")
-    _not_an_input((dq, dk, dv, dbias), (q, k, v, out, stat, dout, kv_len, mask, bias), "cross_attn_bwd")
-    a.dout, a.dq, a.dk, a.dv = dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
-    a.dout_s, a.dq_s, a.dk_s, a.dv_s = _strides3(dout), _strides3(dq), _strides3(dk), _strides3(dv)
+    _on_device(q, k, v, out, stat, dout, dq, dk, dv, dbias, kv_len, mask, bias)
     lib = hip.lib()
-    nws = lib.marship_cross_attn_ws(ctypes.byref(a), 1)
+
+    def build():
+        _req(stat is not None, "cross_attn_bwd: stat of the forward call is needed")
+        a = _cross_block("cross_attn_bwd", q, k, v, out, stat, scale, kv_len, mask, bias)
+        _rows16("cross_attn_bwd", dout=dout, dq=dq, dk=dk, dv=dv)
+        _req(all(t.dtype == q.dtype for t in (dout, dq, dk, dv)), "cross_attn_bwd: one dtype, f32 or bf16")
+        _req(dout.shape == q.shape and dq.shape == q.shape and dk.shape == k.shape and dv.shape == v.shape, "cross_attn_bwd: shape mismatch")
+        if dbias is not None:
+            _req(bias is not None, "cross_attn_bwd: a gradient of a bias that is not there")
+            _req(dbias.dtype == torch.float32 and dbias.shape == bias.shape and (dbias.stride(2) == 1 or dbias.shape[2] == 1),
+                 "cross_attn_bwd: dbias must be f32 [H, Lq, Lk]")
+            _own_elements(dbias, "cross_attn_bwd")
+            a.dbias_s = _strides2(dbias)
+        for t in (dq, dk, dv):
+            _own_elements(t, "cross_attn_bwd")
+        a.dout_s, a.dq_s, a.dk_s, a.dv_s = _strides3(dout), _strides3(dq), _strides3(dk), _strides3(dv)
+        return bytes(a), lib.marship_cross_attn_ws(ctypes.byref(a), 1)
+
+    block, nws = _plan((2, scale, _lay(q), _lay(k), _lay(v), _lay(out), _lay(stat), _lay(dout), _lay(dq), _lay(dk), _lay(dv), _lay(dbias), _lay(kv_len),
+                        _lay(mask), _lay(bias)), build)
+    pq, pk, pv, po, ps = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), stat.data_ptr()
+    pdo, pdq, pdk, pdv, pdb = dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _addr(dbias)
+    _req((pq | pk | pv | po | pdo | pdq | pdk | pdv) % 16 == 0, "cross_attn_bwd: rows must be 16-byte aligned")
+    pb, pl, pm = _addr(bias), _addr(kv_len), _addr(mask)
+    ins, outs = {pq, pk, pv, po, ps, pdo, pb, pl, pm}, [p for p in (pdq, pdk, pdv, pdb) if p]
+    _req(ins.isdisjoint(outs) and len(set(outs)) == len(outs), "cross_attn_bwd: an output lies on another operand")
+    buf = bytearray(block)
+    _PTRS8.pack_into(buf, 0, pq, pk, pv, po, ps, pb, pl, pm)
+    _PTRS5.pack_into(buf, _OFF_BWD, pdo, pdq, pdk, pdv, pdb)
     ws = _workspace(nws, q.device)
-    a.ws, a.ws_bytes = ws.data_ptr(), nws
-    hip.check(lib.marship_cross_attn_bwd(ctypes.byref(a), stream()), "marship_cross_attn_bwd")
+    _PTRS2.pack_into(buf, _OFF_WS, ws.data_ptr(), nws)
+    hip.check(lib.marship_cross_attn_bwd(ctypes.byref(MarsCrossAttn.from_buffer(buf)), stream()), "marship_cross_attn_bwd")
 
 
 def bucket_map(n_q: int, n_k: int, buckets: int, reach: int, *, offset: int = 0, bidirectional: bool = True) -> torch.Tensor:
@@ -1163,7 +1214,6 @@ def bucket_map(n_q: int, n_k: int, buckets: int, reach: int, *, offset: int = 0,
 
 
 def _bias_args(what, table, by, bx, bias, q_grid, k_grid):
-    _dev(table, by, bx, bias)
     (qh, qw), (kh, kw) = q_grid, k_grid
     _req(min(qh, qw, kh, kw) > 0, f"{what}: empty grid")
     _req(table.dim() == 3 and table.is_contiguous() and table.dtype == torch.float32 and table.numel() > 0, f"{what}: table must be contiguous f32 [ny, nx, H]")
@@ -1183,8 +1233,15 @@ def bucket_bias(table: torch.Tensor, by: torch.Tensor, bx: torch.Tensor, out: to
     ``q_grid`` = (qh, qw) and key tokens on ``k_grid`` = (kh, kw), for ``cross_attn``.  table f32 [ny, nx, H]; by, bx i32 on the device, made by ``bucket_map``
     or by any other rule (an entry outside the table: no bias); a line of tokens is a grid of one row with by = [0].  out f32 [H, qh qw, kh kw], rows may be
     wider."""
-    ny, nx, H, s_head, s_row = _bias_args("bucket_bias", table, by, bx, out, q_grid, k_grid)
-    _own_elements(out, "bucket_bias")
+    _on_device(table, by, bx, out)
+
+    def build():
+        args = _bias_args("bucket_bias", table, by, bx, out, q_grid, k_grid)
+        _own_elements(out, "bucket_bias")
+        return args
+
+    ny, nx, H, s_head, s_row = _plan((3, _lay(table), _lay(by), _lay(bx), _lay(out), tuple(q_grid), tuple(k_grid)), build)
+    _req(out.data_ptr() not in (table.data_ptr(), by.data_ptr(), bx.data_ptr()), "bucket_bias: an output lies on another operand")
     hip.check(hip.lib().marship_bucket_bias(ptr(table), ptr(by), ptr(bx), ptr(out), s_head, s_row, H, *q_grid, *k_grid, ny, nx, stream()),
               "marship_bucket_bias")
 
@@ -1192,16 +1249,21 @@ def bucket_bias(table: torch.Tensor, by: torch.Tensor, bx: torch.Tensor, out: to
 def bucket_bias_bwd(dbias: torch.Tensor, by: torch.Tensor, bx: torch.Tensor, dtable: torch.Tensor, *, q_grid, k_grid):
     """dtable f32 [ny, nx, H] = sums of dbias f32 [H, qh qw, kh kw] over the pairs of each bucket: the gradient of ``bucket_bias``.  Every entry is written; sums
     have a fixed order."""
-    ny, nx, H, s_head, s_row = _bias_args("bucket_bias_bwd", dtable, by, bx, dbias, q_grid, k_grid)
+    _on_device(dbias, by, bx, dtable)
     lib = hip.lib()
-    nws = lib.marship_bucket_bias_bwd_ws(H, *q_grid, *k_grid, nx)
+
+    def build():
+        args = _bias_args("bucket_bias_bwd", dtable, by, bx, dbias, q_grid, k_grid)
+        return args + (lib.marship_bucket_bias_bwd_ws(args[2], *q_grid, *k_grid, args[1]),)
+
+    ny, nx, H, s_head, s_row, nws = _plan((4, _lay(dtable), _lay(by), _lay(bx), _lay(dbias), tuple(q_grid), tuple(k_grid)), build)
+    _req(dtable.data_ptr() not in (dbias.data_ptr(), by.data_ptr(), bx.data_ptr()), "bucket_bias_bwd: an output lies on another operand")
     ws = _workspace(nws, dbias.device)
     hip.check(lib.marship_bucket_bias_bwd(ptr(dbias), s_head, s_row, ptr(by), ptr(bx), ptr(dtable), H, *q_grid, *k_grid, ny, nx, ptr(ws), nws, stream()),
               "marship_bucket_bias_bwd")
 
 
 def _norm_args(what, groups, act, w, b, **maps):
-    _dev(w, b, *maps.values())
     x = maps["x"]
     _req(x.dim() == 3 and x.numel() > 0, f"{what}: x must be [N, P, C]")
     N, P, C = x.shape
@@ -1220,35 +1282,49 @@ def group_norm_act(x: torch.Tensor, w: torch.Tensor, b: torch.Tensor, out: torch
     """out = act(GroupNorm(x)) for channels-last maps x [N, P, C] (P pixels or tokens; rows may be wider than C), f32 or bf16 in and out; act is one of
     ``hip.ACT_NONE / ACT_GELU / ACT_QUICKGELU / ACT_RELU / ACT_SILU``.  ``stat`` f32 [N, groups, 2] receives mean and 1 / sqrt(var + eps), which
     ``group_norm_act_bwd`` needs.  out may be x itself."""
-    N, P, C = _norm_args("group_norm_act", groups, act, w, b, x=x, out=out)
-    _own_elements(out, "group_norm_act")
-    _req(eps >= 0.0, "group_norm_act: eps")
-    if stat is not None:
-        _dev(stat)
-        _req(stat.dtype == torch.float32 and stat.is_contiguous() and tuple(stat.shape) == (N, groups, 2), "group_norm_act: stat must be contiguous f32 [N, groups, 2]")
+    _on_device(x, w, b, out, stat)
     lib = hip.lib()
-    nws = lib.marship_group_norm_act_ws(N, P, C, groups, 0)
+
+    def build():
+        N, P, C = _norm_args("group_norm_act", groups, act, w, b, x=x, out=out)
+        _own_elements(out, "group_norm_act")
+        _req(eps >= 0.0, "group_norm_act: eps")
+        _req(stat is None or (stat.dtype == torch.float32 and stat.is_contiguous() and tuple(stat.shape) == (N, groups, 2)),
+             "group_norm_act: stat must be contiguous f32 [N, groups, 2]")
+        return N, P, C, dt(x), dt(out), lib.marship_group_norm_act_ws(N, P, C, groups, 0)
+
+    N, P, C, dtx, dto, nws = _plan((5, groups, eps, act, _lay(x), _lay(w), _lay(b), _lay(out), _lay(stat)), build)
     ws = _workspace(nws, x.device)
-    hip.check(lib.marship_group_norm_act(ptr(x), x.stride(0), x.stride(1), ptr(w), ptr(b), ptr(out), out.stride(0), out.stride(1), N, P, C, groups, eps, act,
-                                         dt(x), dt(out), ptr(stat), ptr(ws), nws, stream()), "marship_group_norm_act")
+    sx, so = x.stride(), out.stride()
+    px, po, ps = x.data_ptr(), out.data_ptr(), _addr(stat)
+    _req(po not in (w.data_ptr(), b.data_ptr()) and ps not in (px, po), "group_norm_act: an output lies on another operand")
+    _req(po != px or (sx == so and dtx == dto), "group_norm_act: in place, out must be x itself")
+    hip.check(lib.marship_group_norm_act(px, sx[0], sx[1], w.data_ptr(), b.data_ptr(), po, so[0], so[1], N, P, C, groups, eps, act, dtx, dto, ps or None,
+                                         ws.data_ptr(), nws, stream()), "marship_group_norm_act")
 
 
 def group_norm_act_bwd(x: torch.Tensor, w: torch.Tensor, b: torch.Tensor, stat: torch.Tensor, dy: torch.Tensor, dx: torch.Tensor, dw: torch.Tensor,
                        db: torch.Tensor, groups: int, act: int = 0):
     """Gradients of ``group_norm_act``: dx [N, P, C] in x's dtype, dw and db f32 [C], from x, the parameters, the forward call's ``stat`` and the gradient dy of
     the output.  dx may be dy itself.  Sums have a fixed order."""
-    N, P, C = _norm_args("group_norm_act_bwd", groups, act, w, b, x=x, dy=dy, dx=dx)
-    _req(dx.dtype == x.dtype, "group_norm_act_bwd: dx must have x's dtype")
-    _own_elements(dx, "group_norm_act_bwd")
-    _dev(stat, dw, db)
-    _req(stat.dtype == torch.float32 and stat.is_contiguous() and tuple(stat.shape) == (N, groups, 2),
-         "group_norm_act_bwd: stat must be contiguous f32 [N, groups, 2]")
-    for name, t in (("dw", dw), ("db", db)):
-        _req(t.dtype == torch.float32 and t.is_contiguous() and tuple(t.shape) == (C,), f"group_norm_act_bwd: {name} must be contiguous f32 [C]")
-    _not_an_input((dw, db), (x, w, b, stat, dy, dx), "group_norm_act_bwd")
+    _on_device(x, w, b, stat, dy, dx, dw, db)
     lib = hip.lib()
-    nws = lib.marship_group_norm_act_ws(N, P, C, groups, 1)
+
+    def build():
+        N, P, C = _norm_args("group_norm_act_bwd", groups, act, w, b, x=x, dy=dy, dx=dx)
+        _req(dx.dtype == x.dtype, "group_norm_act_bwd: dx must have x's dtype")
+        _own_elements(dx, "group_norm_act_bwd")
+        _req(stat.dtype == torch.float32 and stat.is_contiguous() and tuple(stat.shape) == (N, groups, 2),
+             "group_norm_act_bwd: stat must be contiguous f32 [N, groups, 2]")
+        for name, t in (("dw", dw), ("db", db)):
+            _req(t.dtype == torch.float32 and t.is_contiguous() and tuple(t.shape) == (C,), f"group_norm_act_bwd: {name} must be contiguous f32 [C]")
+        return N, P, C, dt(x), dt(dy), lib.marship_group_norm_act_ws(N, P, C, groups, 1)
+
+    N, P, C, dtx, dty, nws = _plan((6, groups, act, _lay(x), _lay(w), _lay(b), _lay(stat), _lay(dy), _lay(dx), _lay(dw), _lay(db)), build)
+    sx, sy, sd = x.stride(), dy.stride(), dx.stride()
+    px, pw, pb, ps, py, pd, pdw, pdb = (t.data_ptr() for t in (x, w, b, stat, dy, dx, dw, db))
+    _req(len({pdw, pdb, pd} | {px, pw, pb, ps}) == 3 + len({px, pw, pb, ps}) and py not in (pdw, pdb), "group_norm_act_bwd: an output lies on another operand")
+    _req(pd != py or (sd == sy and dtx == dty), "group_norm_act_bwd: in place, dx must be dy itself")
     ws = _workspace(nws, x.device)
-    hip.check(lib.marship_group_norm_act_bwd(ptr(x), x.stride(0), x.stride(1), ptr(w), ptr(b), ptr(stat), ptr(dy), dy.stride(0), dy.stride(1), ptr(dx),
-                                             dx.stride(0), dx.stride(1), ptr(dw), ptr(db), N, P, C, groups, act, dt(x), dt(dy), ptr(ws), nws, stream()),
-              "marship_group_norm_act_bwd")
+    hip.check(lib.marship_group_norm_act_bwd(px, sx[0], sx[1], pw, pb, ps, py, sy[0], sy[1], pd, sd[0], sd[1], pdw, pdb, N, P, C, groups, act, dtx, dty,
+                                             ws.data_ptr(), nws, stream()), "marship_group_norm_act_bwd")
