@@ -216,7 +216,7 @@ int marship_cross_attn_bwd(const MarsCrossAttn* args, void* stream);
  * marship_bucket_bias_bwd_ws bytes, 16-byte aligned. */
 int marship_bucket_bias(const float* table, const int32_t* by, const int32_t* bx, float* out, int64_t s_head, int64_t s_row, int H, int qh, int qw,
                         int kh, int kw, int ny, int nx, void* stream);
-int64_t marship_bucket_bias_bwd_ws(int H, int qh, int qw, int kh, int kw, int nx);
+int64_t marship_bucket_bias_bwd_ws(int H, int qh, int qw, int kh, int kw, int ny, int nx);
 int marship_bucket_bias_bwd(const float* dbias, int64_t s_head, int64_t s_row, const int32_t* by, const int32_t* bx, float* dtable, int H, int qh,
                             int qw, int kh, int kw, int ny, int nx, void* ws, int64_t ws_bytes, void* stream);
 

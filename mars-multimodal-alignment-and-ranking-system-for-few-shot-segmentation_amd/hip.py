@@ -132,7 +132,7 @@ _SIGNATURES = {
     "marship_cross_attn": [POINTER(MarsCrossAttn), _P],
     "marship_cross_attn_bwd": [POINTER(MarsCrossAttn), _P],
     "marship_bucket_bias": [_P, _P, _P, _P, _L, _L, _I, _I, _I, _I, _I, _I, _I, _P],
-    "marship_bucket_bias_bwd_ws": [_I, _I, _I, _I, _I, _I],
+    "marship_bucket_bias_bwd_ws": [_I, _I, _I, _I, _I, _I, _I],
     "marship_bucket_bias_bwd": [_P, _L, _L, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _L, _P],
     "marship_group_norm_act_ws": [_I, _I, _I, _I, _I],
     "marship_group_norm_act": [_P, _L, _L, _P, _P, _P, _L, _L, _I, _I, _I, _I, _F, _I, _I, _I, _P, _P, _L, _P],

@@ -1254,7 +1254,7 @@ def bucket_bias_bwd(dbias: torch.Tensor, by: torch.Tensor, bx: torch.Tensor, dta
 
     def build():
         args = _bias_args("bucket_bias_bwd", dtable, by, bx, dbias, q_grid, k_grid)
-        return args + (lib.marship_bucket_bias_bwd_ws(args[2], *q_grid, *k_grid, args[1]),)
+        return args + (lib.marship_bucket_bias_bwd_ws(args[2], *q_grid, *k_grid, args[0], args[1]),)
 
     ny, nx, H, s_head, s_row, nws = _plan((4, _lay(dtable), _lay(by), _lay(bx), _lay(dbias), tuple(q_grid), tuple(k_grid)), build)
     _req(dtable.data_ptr() not in (dbias.data_ptr(), by.data_ptr(), bx.data_ptr()), "bucket_bias_bwd: an output lies on another operand")
