@@ -19,8 +19,12 @@ typedef float f32x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
+typedef __attribute__((address_space(3))) unsigned char* lds_t;          // a tile in LDS
 typedef const __attribute__((address_space(1))) void* gbl_ptr_t;
 typedef __attribute__((address_space(3))) s16x4* lds_s16x4_t;
+typedef const __attribute__((address_space(3))) bf16x8* lds_bf16x8_t;
+typedef const __attribute__((address_space(3))) f32x4* lds_f32x4_t;
+typedef const __attribute__((address_space(3))) float* lds_f32_t;
 
 static __device__ uint4 zero_chunk;          // 16 bytes of zeros: what a fill reads behind the end of a row
 
@@ -88,7 +92,7 @@ template <typename T, int HDP> struct Tile {
         static __device__ __forceinline__ int row_of_fill(int i, int w, int lane) { return ((w + i * NW) * 64 + lane) / LPR; }
         // at(i): the first byte of fill i's row; hdb: bytes of a row that exist (the rest is zeros).  Straight-line code: a branch or a wait
         // between two fills would hold up the later ones by a trip to memory
-        template <typename F> static __device__ __forceinline__ void run(unsigned char* dst, int w, int lane, int hdb, F at) {
+        template <typename F> static __device__ __forceinline__ void run(lds_t dst, int w, int lane, int hdb, F at) {
             const unsigned char* zeros = (const unsigned char*)&zero_chunk;
 #pragma unroll
             for (int i = 0; i < FILLS; ++i) {
@@ -103,19 +107,19 @@ template <typename T, int HDP> struct Tile {
         }
     };
     // fragment of rows r0 + (lane & 31), contraction step ks over the row's elements
-    static __device__ __forceinline__ frag_t<T> rows(const unsigned char* t, int r0, int ks, int lane) {
+    static __device__ __forceinline__ frag_t<T> rows(lds_t t, int r0, int ks, int lane) {
         const int row = r0 + (lane & 31), hh = lane >> 5, sw = swizzle(row);
         if constexpr (sizeof(T) == 2) {
-            return __builtin_bit_cast(bf16x8, *(const uint4*)(t + row * ROWB + (((2 * ks + hh) ^ sw) << 4)));
+            return *(lds_bf16x8_t)(t + row * ROWB + (((2 * ks + hh) ^ sw) << 4));
         } else {
-            const f32x4 a = *(const f32x4*)(t + row * ROWB + (((4 * ks + 2 * hh) ^ sw) << 4));
-            const f32x4 b = *(const f32x4*)(t + row * ROWB + (((4 * ks + 2 * hh + 1) ^ sw) << 4));
+            const f32x4 a = *(lds_f32x4_t)(t + row * ROWB + (((4 * ks + 2 * hh) ^ sw) << 4));
+            const f32x4 b = *(lds_f32x4_t)(t + row * ROWB + (((4 * ks + 2 * hh + 1) ^ sw) << 4));
             return (f32x8){a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
         }
     }
     // fragment of columns 32 m + (lane & 31): its elements are rows r0 + 8 (e >> 2) + 4 (lane >> 5) + (e & 3), the rows that pack_step's
     // registers belong to
-    static __device__ __forceinline__ frag_t<T> cols(const unsigned char* t, int r0, int m, int lane) {
+    static __device__ __forceinline__ frag_t<T> cols(lds_t t, int r0, int m, int lane) {
         const int hh = lane >> 5;
         if constexpr (sizeof(T) == 2) {
             // ds_read_b64_tr_b16: sixteen lanes read four rows of sixteen 16-bit columns and each gets one column
@@ -130,7 +134,7 @@ template <typename T, int HDP> struct Tile {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const int row = r0 + 8 * (e >> 2) + 4 * hh + (e & 3);
-                r[e] = *(const float*)(t + row * ROWB + ((chunk ^ swizzle(row)) << 4) + 4 * (d & 3));
+                r[e] = *(lds_f32_t)(t + row * ROWB + ((chunk ^ swizzle(row)) << 4) + 4 * (d & 3));
             }
             return r;
         }

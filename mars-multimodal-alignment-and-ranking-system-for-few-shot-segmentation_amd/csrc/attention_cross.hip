@@ -119,7 +119,7 @@ __global__ __launch_bounds__(256, (FwdCfg<T, HDP, FEW>::WPE)) void cross_fwd_ker
         }
     };
     // fills of tile t, whose rows are looked up; then the rows of the next one
-    auto issue = [&](int t, unsigned char* dst) {
+    auto issue = [&](int t, lds_t dst) {
         FL::run(dst, fw, lane, hdb, [&](int i) { return kbase + rows[i] * kl; });
         FL::run(dst + TB, fw, lane, hdb, [&](int i) { return vbase + rows[i] * vl; });
         look_up(t + STEP);
@@ -136,7 +136,7 @@ __global__ __launch_bounds__(256, (FwdCfg<T, HDP, FEW>::WPE)) void cross_fwd_ker
     // a mask made of the type's lowest value would overflow in units of log 2.
     // next(): the fills of a later tile, issued behind this tile's bias loads (loads come back in order: the other way round the first use of
     // the bias would wait for the fills)
-    auto tile_of = [&](auto whole_tag, int t, const unsigned char* kt, const unsigned char* vt, auto next) {
+    auto tile_of = [&](auto whole_tag, int t, lds_t kt, lds_t vt, auto next) {
         constexpr bool WHOLE = decltype(whole_tag)::value;
         f32x16 s[KB];
         float bias[BIAS ? KB : 1][16];
@@ -204,42 +204,41 @@ __global__ __launch_bounds__(256, (FwdCfg<T, HDP, FEW>::WPE)) void cross_fwd_ker
     constexpr std::false_type ragged{};
     auto nothing = [] {};
 
+    const lds_t my0 = (lds_t)buf0[cw][0], my1 = Cfg::BUFS == 2 ? (lds_t)buf1[Cfg::BUFS == 2 ? cw : 0][0] : my0;
     if constexpr (!FEW) {
         look_up(t0);
-        if (t0 < t1) issue(t0, buf0[0][0]);
+        if (t0 < t1) issue(t0, my0);
         int t = t0;
         if constexpr (Cfg::BUFS == 2) {
             bool odd = false;
             while (t < tw) {
                 tile_barrier();
-                tile_of(whole, t, buf0[0][0], buf0[0][1], [&] { if (t + 1 < t1) issue(t + 1, buf1[0][0]); });
+                tile_of(whole, t, my0, my0 + TB, [&] { if (t + 1 < t1) issue(t + 1, my1); });
                 odd = true;
                 if (++t >= tw) break;
                 tile_barrier();
-                tile_of(whole, t, buf1[0][0], buf1[0][1], [&] { if (t + 1 < t1) issue(t + 1, buf0[0][0]); });
+                tile_of(whole, t, my1, my1 + TB, [&] { if (t + 1 < t1) issue(t + 1, my0); });
                 odd = false;
                 ++t;
             }
             if (t < t1) {
                 tile_barrier();
-                const unsigned char* at = odd ? buf1[0][0] : buf0[0][0];
+                const lds_t at = odd ? my1 : my0;
                 tile_of(ragged, t, at, at + TB, nothing);
             }
         } else {
             for (; t < tw; ++t) {
                 tile_barrier();
-                tile_of(whole, t, buf0[0][0], buf0[0][1], nothing);
+                tile_of(whole, t, my0, my0 + TB, nothing);
                 tile_barrier();
-                if (t + 1 < t1) issue(t + 1, buf0[0][0]);
+                if (t + 1 < t1) issue(t + 1, my0);
             }
             if (t < t1) {
                 tile_barrier();
-                tile_of(ragged, t, buf0[0][0], buf0[0][1], nothing);
+                tile_of(ragged, t, my0, my0 + TB, nothing);
             }
         }
     } else {
-        unsigned char* my0 = buf0[cw][0];
-        unsigned char* my1 = Cfg::BUFS == 2 ? buf1[Cfg::BUFS == 2 ? cw : 0][0] : my0;
         // a wave's own buffers need its own waits only
         int t = t0 + wave;
         look_up(t);
@@ -259,7 +258,7 @@ __global__ __launch_bounds__(256, (FwdCfg<T, HDP, FEW>::WPE)) void cross_fwd_ker
             }
             if (t < t1) {
                 __builtin_amdgcn_s_waitcnt(0);
-                const unsigned char* at = odd ? my1 : my0;
+                const lds_t at = odd ? my1 : my0;
                 tile_of(ragged, t, at, at + TB, nothing);
             }
         } else {
@@ -472,6 +471,7 @@ int check(const MarsCrossAttn* a, bool backward) {
     MARS_CHECK(a->hd > 0 && a->hd <= 128 && (a->hd * es) % 16 == 0, "%s: head dim %d (up to 128, a multiple of 16 bytes)", what, a->hd);
     MARS_CHECK((int64_t)(a->H / a->Hkv) * a->Lq < (1ll << 30) && a->Lk < (1 << 30), "%s: too many rows", what);
     MARS_CHECK((int64_t)a->B * a->H < (1ll << 30), "%s: too many heads", what);
+    MARS_CHECK(a->bias == nullptr || (a->bias_s[1] >= 0 && a->bias_s[1] < (1 << 28)), "%s: bias rows too far apart", what);
     MARS_CHECK(a->scale > 0.f && a->scale < INFINITY, "%s: scale must be positive and finite", what);
     MARS_CHECK(rows_ok(a->q, a->q_s, es) && rows_ok(a->k, a->k_s, es) && rows_ok(a->v, a->v_s, es) && rows_ok(a->out, a->out_s, es),
                "%s: rows must be 16-byte aligned", what);

@@ -29,7 +29,10 @@ namespace {
 // and factor = 1 / sum: where the mask is the type's lowest value the sum's logarithm would be lost in the maximum.
 // Rows that do not exist or have no key: P = 0.
 constexpr int RSB = 128;
-constexpr int QW = 96, KW = 96;
+// waves a SIMD that the two passes are built for (three of the key pass's would spill: 109 -> 142 us on eight 1369 x 684 x 16 heads of 64; the query
+// pass with three, walking tiles of 32 keys: 98 -> 89)
+template <typename T, int HDP, bool BIAS> constexpr int q_waves() { return sizeof(T) == 4 || HDP > 96 ? 1 : HDP > 64 || BIAS ? 2 : 3; }
+template <typename T, int HDP> constexpr int kv_waves() { return sizeof(T) == 4 || HDP > 96 ? 1 : 2; }
 
 struct Bwd {
     Prob p;
@@ -51,9 +54,9 @@ template <bool BIAS> __device__ __forceinline__ float prob(float s, float c2, fl
 }
 
 template <typename T, int HDP, bool BIAS>
-__global__ __launch_bounds__(256, (HDP <= QW && sizeof(T) == 2) ? 2 : 1) void cross_bwd_q_kernel(const Bwd f) {
+__global__ __launch_bounds__(256, (q_waves<T, HDP, BIAS>())) void cross_bwd_q_kernel(const Bwd f) {
     using TL = Tile<T, HDP>;
-    constexpr int KT = (HDP > 64 && sizeof(T) == 4) ? 32 : 64, TB = KT * TL::ROWB, KB = KT / 32, KS = HDP / 16, DM = HDP / 32;
+    constexpr int KT = (HDP > 64 && sizeof(T) == 4) || q_waves<T, HDP, BIAS>() == 3 ? 32 : 64, TB = KT * TL::ROWB, KB = KT / 32, KS = HDP / 16, DM = HDP / 32;
     __shared__ __attribute__((aligned(16))) unsigned char buf0[2][TB];
     __shared__ __attribute__((aligned(16))) unsigned char buf1[2][TB];
     const Prob& p = f.p;
@@ -84,15 +87,16 @@ __global__ __launch_bounds__(256, (HDP <= QW && sizeof(T) == 2) ? 2 : 1) void cr
             for (int i = 0; i < FL::FILLS; ++i) rows[i] = idx[rows[i]];
         }
     };
-    auto issue = [&](int t, unsigned char (&dst)[2][TB]) {
-        FL::run(dst[0], wave, lane, hdb, [&](int i) { return kbase + rows[i] * kl; });
-        FL::run(dst[1], wave, lane, hdb, [&](int i) { return vbase + rows[i] * vl; });
+    auto issue = [&](int t, lds_t dst) {
+        FL::run(dst, wave, lane, hdb, [&](int i) { return kbase + rows[i] * kl; });
+        FL::run(dst + TB, wave, lane, hdb, [&](int i) { return vbase + rows[i] * vl; });
         look_up(t + 1);
     };
     int t0, t1;
     split_range((n + KT - 1) / KT, split, f.nsq, t0, t1);
     look_up(t0);
-    if (t0 < t1) issue(t0, buf0);
+    const lds_t b0 = (lds_t)buf0[0], b1 = (lds_t)buf1[0];
+    if (t0 < t1) issue(t0, b0);
 
     frag_t<T> qf[KS], dof[KS];
     const T* qrow = row_ok ? row_ptr<T>(p.q, p.sq, b, l, h) : nullptr;
@@ -126,7 +130,7 @@ __global__ __launch_bounds__(256, (HDP <= QW && sizeof(T) == 2) ? 2 : 1) void cr
     for (int m = 0; m < DM; ++m) dq[m] = zero16();
 #pragma unroll
     for (int m = 0; m < (MEND ? DM : 1); ++m) pk[m] = zero16();
-    auto tile_of = [&](auto whole_tag, int t, const unsigned char* kt, const unsigned char* vt, auto next) {
+    auto tile_of = [&](auto whole_tag, int t, lds_t kt, lds_t vt, auto next) {
         constexpr bool WHOLE = decltype(whole_tag)::value;
         float bias[BIAS ? KB : 1][16];
         if constexpr (BIAS) {
@@ -173,17 +177,17 @@ __global__ __launch_bounds__(256, (HDP <= QW && sizeof(T) == 2) ? 2 : 1) void cr
     bool odd = false;
     while (t < tw) {
         tile_barrier();
-        tile_of(std::true_type{}, t, buf0[0], buf0[1], [&] { if (t + 1 < t1) issue(t + 1, buf1); });
+        tile_of(std::true_type{}, t, b0, b0 + TB, [&] { if (t + 1 < t1) issue(t + 1, b1); });
         odd = true;
         if (++t >= tw) break;
         tile_barrier();
-        tile_of(std::true_type{}, t, buf1[0], buf1[1], [&] { if (t + 1 < t1) issue(t + 1, buf0); });
+        tile_of(std::true_type{}, t, b1, b1 + TB, [&] { if (t + 1 < t1) issue(t + 1, b0); });
         odd = false;
         ++t;
     }
     if (t < t1) {
         tile_barrier();
-        const unsigned char* at = odd ? buf1[0] : buf0[0];
+        const lds_t at = odd ? b1 : b0;
         tile_of(std::false_type{}, t, at, at + TB, [] {});
     }
     if constexpr (MEND) e = halves_sum(e);
@@ -232,7 +236,7 @@ template <typename T, int HDP> struct KeyCfg {
 };
 
 template <typename T, int HDP, bool BIAS>
-__global__ __launch_bounds__(256, (HDP <= KW && sizeof(T) == 2) ? 2 : 1) void cross_bwd_kv_kernel(const Bwd f) {
+__global__ __launch_bounds__(256, (kv_waves<T, HDP>())) void cross_bwd_kv_kernel(const Bwd f) {
     using TL = Tile<T, HDP>;
     using Cfg = KeyCfg<T, HDP>;
     constexpr int QT = Cfg::QT, TB = Cfg::TB, KS = HDP / 16, DM = HDP / 32;
@@ -269,7 +273,7 @@ __global__ __launch_bounds__(256, (HDP <= KW && sizeof(T) == 2) ? 2 : 1) void cr
         const unsigned char* dobase = (const unsigned char*)row_ptr<T>(p.dout, p.sdo, b, 0, 0);
         using FL = typename TL::template Fill<QT, 4>;
         // (rows behind the last one: that one again - their P is 0)
-        auto issue = [&](int t, unsigned char* dst) {
+        auto issue = [&](int t, lds_t dst) {
             int64_t oq[FL::FILLS], od[FL::FILLS];
 #pragma unroll
             for (int i = 0; i < FL::FILLS; ++i) {
@@ -285,21 +289,29 @@ __global__ __launch_bounds__(256, (HDP <= KW && sizeof(T) == 2) ? 2 : 1) void cr
                 __builtin_amdgcn_global_load_lds((gbl_ptr_t)(rows + (int64_t)t * (QT / 32) * RSB + 4 * lane), (lds_ptr_t)(dst + 2 * TB), 16, 0, 0);
         };
         const float c2 = p.scale * LOG2E;
-        const float* bcol = BIAS && attended ? p.bias + key : nullptr;
-        auto tile = [&](int t, const unsigned char* base, auto next) {
-            const unsigned char *qt = base, *dot = base + TB;
+        const unsigned blane = BIAS ? (unsigned)(4 * hh * p.bias_l) + key : 0;      // (a lane whose key is not attended reads its bias too: its column is not used)
+        auto tile = [&](int t, lds_t base, auto next) {
+            const lds_t qt = base, dot = base + TB;
 #pragma unroll
             for (int qb = 0; qb < QT / 32; ++qb) {
-                const float* rs = (const float*)(base + 2 * TB) + qb * RSB;
+                const lds_f32_t rs = (lds_f32_t)(base + 2 * TB) + qb * RSB;
                 float bias[16];
                 if constexpr (BIAS) {
                     const int r0 = t * QT + 32 * qb;
+                    int l0, h0;
+                    row_of(p, hk, min(r0, p.R - 1), l0, h0);
+                    if (l0 + 32 <= p.Lq) {                          // 32 rows of one head: whole-wave row addresses, the lanes' part in 32 bits
+                        const float* base = p.bias + h0 * p.bias_h + l0 * p.bias_l;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int r = r0 + acc_row(i, hh);
-                        int l, h;
-                        row_of(p, hk, min(r, p.R - 1), l, h);
-                        bias[i] = bcol != nullptr && r < p.R ? bcol[h * p.bias_h + l * p.bias_l] : 0.f;
+                        for (int i = 0; i < 16; ++i) bias[i] = (base + (8 * (i >> 2) + (i & 3)) * p.bias_l)[blane];
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const int r = r0 + acc_row(i, hh);
+                            int l, h;
+                            row_of(p, hk, min(r, p.R - 1), l, h);
+                            bias[i] = r < p.R ? p.bias[h * p.bias_h + l * p.bias_l + key] : 0.f;
+                        }
                     }
                 }
                 if (qb == 0) next();
@@ -311,9 +323,9 @@ __global__ __launch_bounds__(256, (HDP <= KW && sizeof(T) == 2) ? 2 : 1) void cr
                 }
 #pragma unroll
                 for (int a = 0; a < 4; ++a) {
-                    const f32x4 off = *(const f32x4*)(rs + 8 * a + 4 * hh), D = *(const f32x4*)(rs + 64 + 8 * a + 4 * hh);
+                    const f32x4 off = *(lds_f32x4_t)(rs + 8 * a + 4 * hh), D = *(lds_f32x4_t)(rs + 64 + 8 * a + 4 * hh);
                     f32x4 fac = {1.f, 1.f, 1.f, 1.f};
-                    if constexpr (BIAS) fac = *(const f32x4*)(rs + 32 + 8 * a + 4 * hh);
+                    if constexpr (BIAS) fac = *(lds_f32x4_t)(rs + 32 + 8 * a + 4 * hh);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int i = 4 * a + e;
@@ -334,13 +346,14 @@ __global__ __launch_bounds__(256, (HDP <= KW && sizeof(T) == 2) ? 2 : 1) void cr
                 }
             }
         };
-        if (t0 < t1) issue(t0, buf0);
+        const lds_t b0 = (lds_t)buf0, b1 = (lds_t)buf1;
+        if (t0 < t1) issue(t0, b0);
         for (int t = t0; t < t1; t += 2) {
             tile_barrier();
-            tile(t, buf0, [&] { if (t + 1 < t1) issue(t + 1, buf1); });
+            tile(t, b0, [&] { if (t + 1 < t1) issue(t + 1, b1); });
             if (t + 1 < t1) {
                 tile_barrier();
-                tile(t + 1, buf1, [&] { if (t + 2 < t1) issue(t + 2, buf0); });
+                tile(t + 1, b1, [&] { if (t + 2 < t1) issue(t + 2, b0); });
             }
         }
     }
@@ -460,7 +473,7 @@ __global__ __launch_bounds__(256, (HDP <= 64 && sizeof(T) == 2) ? 2 : 1) void cr
     frag_t<T> qf[KS], dof[KS];
     float off = 0.f, fac = 0.f, D = 0.f;
     bool on[2];
-    auto fetch = [&](int b, unsigned char (&dst)[2][TB]) {
+    auto fetch = [&](int b, lds_t dst) {
         const int len = length(b);
         const T* qrow = row_ptr<T>(p.q, p.sq, b, l, h);
         const T* dorow = row_ptr<T>(p.dout, p.sdo, b, l, h);
@@ -478,11 +491,11 @@ __global__ __launch_bounds__(256, (HDP <= 64 && sizeof(T) == 2) ? 2 : 1) void cr
         const unsigned char* kbase = (const unsigned char*)row_ptr<T>(p.k, p.sk, b, 0, hk);
         const unsigned char* vbase = (const unsigned char*)row_ptr<T>(p.v, p.sv, b, 0, hk);
         using FL = typename TL::template Fill<KT, 4>;
-        FL::run(dst[0], wave, lane, hdb, [&](int i) { return kbase + min(j0 + FL::row_of_fill(i, wave, lane), len - 1) * p.sk.l * (int)sizeof(T); });
-        FL::run(dst[1], wave, lane, hdb, [&](int i) { return vbase + min(j0 + FL::row_of_fill(i, wave, lane), len - 1) * p.sv.l * (int)sizeof(T); });
+        FL::run(dst, wave, lane, hdb, [&](int i) { return kbase + min(j0 + FL::row_of_fill(i, wave, lane), len - 1) * p.sk.l * (int)sizeof(T); });
+        FL::run(dst + TB, wave, lane, hdb, [&](int i) { return vbase + min(j0 + FL::row_of_fill(i, wave, lane), len - 1) * p.sv.l * (int)sizeof(T); });
     };
     // one entry: its tiles are in cur; returns the entry whose fetch into the other buffer it started
-    auto work = [&](int b, unsigned char (&cur)[2][TB], unsigned char (&other)[2][TB]) {
+    auto work = [&](int b, lds_t cur, lds_t other) {
         rowv[wave][0][lane & 31] = off;                             // (both half-waves hold the same rows)
         rowv[wave][1][lane & 31] = fac;
         rowv[wave][2][lane & 31] = D;
@@ -498,8 +511,8 @@ __global__ __launch_bounds__(256, (HDP <= 64 && sizeof(T) == 2) ? 2 : 1) void cr
             f32x16 s = zero16(), dp = zero16();
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                s = mma(q[ks], TL::rows(cur[0], 32 * kb, ks, lane), s);
-                dp = mma(d[ks], TL::rows(cur[1], 32 * kb, ks, lane), dp);
+                s = mma(q[ks], TL::rows(cur, 32 * kb, ks, lane), s);
+                dp = mma(d[ks], TL::rows(cur + TB, 32 * kb, ks, lane), dp);
             }
 #pragma unroll
             for (int a = 0; a < 4; ++a) {
@@ -516,11 +529,12 @@ __global__ __launch_bounds__(256, (HDP <= 64 && sizeof(T) == 2) ? 2 : 1) void cr
         }
         return nb;
     };
+    const lds_t b0 = (lds_t)buf0[0], b1 = (lds_t)buf1[0];
     int b = entry(0);
-    if (b < p.B) fetch(b, buf0);
+    if (b < p.B) fetch(b, b0);
     while (b < p.B) {
-        b = work(b, buf0, buf1);
-        if (b < p.B) b = work(b, buf1, buf0);
+        b = work(b, b0, b1);
+        if (b < p.B) b = work(b, b1, b0);
     }
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
