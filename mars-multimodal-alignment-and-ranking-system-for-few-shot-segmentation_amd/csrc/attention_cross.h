@@ -75,6 +75,11 @@ __device__ __forceinline__ float halves_max(float x) {
     return vmax(__builtin_bit_cast(float, (unsigned)r[0]), __builtin_bit_cast(float, (unsigned)r[1]));
 }
 
+// The kernels are built for head dims HD of 16, 32, 64, 80, 96 and 128; a head is zero-padded to the next of them for the products that contract
+// over it, and to a multiple of 32 (HDP) where its elements are the rows of a product.
+constexpr int padded(int HD) { return (HD + 31) / 32 * 32; }
+inline int built_for(int hd) { return hd <= 16 ? 16 : hd <= 32 ? 32 : hd <= 64 ? 64 : hd <= 80 ? 80 : hd <= 96 ? 96 : 128; }
+
 // ---- LDS tiles: rows of HDP elements in 16-byte chunks, filled by LDS-DMA.  Chunk c of row r sits at slot
 // c ^ swizzle(r): of the rows that a fragment read touches with one chunk number, those whose row starts fall on the same
 // banks (64 banks of 4 bytes) use different slots.

@@ -61,7 +61,8 @@ struct Fwd {
 
 // FEW: at most 32 rows: the four waves share them and take key tiles in turn, each through LDS buffers of its own (no barrier),
 // and join their results at the end.  Otherwise each wave has 32 rows of a 128-row block and the workgroup shares the tiles.
-template <typename T, int HDP, bool FEW> struct FwdCfg {
+template <typename T, int HD, bool FEW> struct FwdCfg {
+    static constexpr int HDP = padded(HD);
     static constexpr int KT = FEW ? 32 : 64;                                             // keys per tile
     static constexpr int TB = KT * HDP * (int)sizeof(T);
     static constexpr int COPIES = FEW ? 4 : 1;
@@ -69,11 +70,12 @@ template <typename T, int HDP, bool FEW> struct FwdCfg {
     static constexpr int WPE = COPIES * BUFS * 2 * TB <= 80 * 1024 ? 2 : 1;              // waves a SIMD that the LDS leaves room for
 };
 
-template <typename T, int HDP, bool BIAS, bool FEW>
-__global__ __launch_bounds__(256, (FwdCfg<T, HDP, FEW>::WPE)) void cross_fwd_kernel(const Fwd f) {
-    using Cfg = FwdCfg<T, HDP, FEW>;
+template <typename T, int HD, bool BIAS, bool FEW>
+__global__ __launch_bounds__(256, (FwdCfg<T, HD, FEW>::WPE)) void cross_fwd_kernel(const Fwd f) {
+    using Cfg = FwdCfg<T, HD, FEW>;
+    constexpr int HDP = Cfg::HDP;
     using TL = Tile<T, HDP>;
-    constexpr int KT = Cfg::KT, TB = Cfg::TB, KB = KT / 32, KS = HDP / 16, DM = HDP / 32;
+    constexpr int KT = Cfg::KT, TB = Cfg::TB, KB = KT / 32, KS = HD / 16, DM = HDP / 32;
     __shared__ __attribute__((aligned(16))) unsigned char buf0[Cfg::COPIES][2][TB];
     __shared__ __attribute__((aligned(16))) unsigned char buf1[Cfg::BUFS == 2 ? Cfg::COPIES : 1][Cfg::BUFS == 2 ? 2 : 1][Cfg::BUFS == 2 ? TB : 16];
     const Prob& p = f.p;
@@ -341,16 +343,17 @@ __global__ __launch_bounds__(256, (FwdCfg<T, HDP, FEW>::WPE)) void cross_fwd_ker
     }
 }
 
-// Joins the splits.  A lane owns four elements of a row, HDP / 4 lanes a row; where the splits outnumber it, 64 / (HDP / 4) lane groups of a wave take the splits
-// of one row in turn (each with its own running maximum) and meet in shuffles: the loads of a row are few trips to memory deep.
-template <typename T, int HDP>
+// Joins the splits.  A lane owns four elements of a row, HDP / 4 lanes a row.  DEEP: the lane groups of a wave take the splits of one row in turn (each with
+// its own running maximum) and meet in shuffles, so that the loads of a row are few trips to memory deep; otherwise (few splits, many rows)
+// each group has a row of its own.
+template <typename T, int HDP, bool DEEP>
 __global__ __launch_bounds__(256) void cross_join_kernel(const Fwd f) {
     constexpr int LR = HDP / 4 == 24 ? 32 : HDP / 4, NG = 64 / LR;          // lanes a row (96: eight of 32 stay idle), groups a wave
     const Prob& p = f.p;
     const int64_t rows = (int64_t)p.B * p.Hkv * p.R;
-    const int lane = threadIdx.x & 63, grp = lane / LR, d = 4 * (lane % LR);
-    const int64_t g = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (g >= rows) return;
+    const int lane = threadIdx.x & 63, grp = lane / LR, d = 4 * (lane % LR), first = DEEP ? grp : 0, step = DEEP ? NG : 1;
+    const int64_t wave = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), g = DEEP ? wave : wave * NG + grp;
+    if (g >= rows) return;                                                  // (DEEP: the whole wave)
     const bool on = d < HDP;
     float m = -INFINITY, l = 0.f;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
@@ -363,12 +366,12 @@ __global__ __launch_bounds__(256) void cross_join_kernel(const Fwd f) {
         m = mn;
     };
     constexpr int U = 4;
-    for (int s0 = grp; s0 < f.ns; s0 += NG * U) {
+    for (int s0 = first; s0 < f.ns; s0 += step * U) {
         float ms[U], ls[U];
         f32x4 v[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int s = s0 + u * NG;
+            const int s = s0 + u * step;
             ms[u] = -INFINITY;
             ls[u] = 0.f;
             v[u] = (f32x4){0.f, 0.f, 0.f, 0.f};
@@ -382,12 +385,12 @@ __global__ __launch_bounds__(256) void cross_join_kernel(const Fwd f) {
         for (int u = 0; u < U; ++u) add(ms[u], ls[u], v[u]);
     }
 #pragma unroll
-    for (int o = LR; o < 64; o <<= 1) {
+    for (int o = DEEP ? LR : 64; o < 64; o <<= 1) {
         const float mo = __shfl_xor(m, o, 64), lo = __shfl_xor(l, o, 64);
         const f32x4 v = {__shfl_xor(acc[0], o, 64), __shfl_xor(acc[1], o, 64), __shfl_xor(acc[2], o, 64), __shfl_xor(acc[3], o, 64)};
         add(mo, lo, v);
     }
-    if (grp != 0) return;
+    if (DEEP && grp != 0) return;
     const int bh = (int)(g / p.R), r = (int)(g - (int64_t)bh * p.R), b = bh / p.Hkv, hk = bh - b * p.Hkv;
     int tok, h;
     row_of(p, hk, r, tok, h);
@@ -401,11 +404,12 @@ __global__ __launch_bounds__(256) void cross_join_kernel(const Fwd f) {
 }
 
 // How a launch is cut: row blocks, and splits of the keys where the row blocks alone leave CUs idle.
-struct FwdPlan { bool few; int hdp, nrb, ns; int64_t part_bytes; };
+struct FwdPlan { bool few; int hd, hdp, nrb, ns; int64_t part_bytes; };
 FwdPlan plan_fwd(const MarsCrossAttn* a) {
     FwdPlan pl;
     const int64_t R = (int64_t)(a->H / a->Hkv) * a->Lq;
-    pl.hdp = (a->hd + 31) / 32 * 32;
+    pl.hd = built_for(a->hd);
+    pl.hdp = padded(pl.hd);
     pl.few = R <= 32;
     pl.nrb = (int)(pl.few ? 1 : (R + 127) / 128);
     const int64_t blocks = (int64_t)a->B * a->Hkv * pl.nrb;
@@ -416,36 +420,52 @@ FwdPlan plan_fwd(const MarsCrossAttn* a) {
         const int most = pl.few ? (tiles + 3) / 4 : (tiles + 1) / 2;             // at least two tiles a wave
         pl.ns = (int)(want < most ? want : most);
         if (pl.ns < 1) pl.ns = 1;
+    } else if (!pl.few && blocks < 1024) {
+        // Little more than a round of workgroups: some CUs work on one more than the others.  Cutting the keys evens that out where it gains more than
+        // the partial results cost (written and read once at memory speed, and a launch) - 1369 queries over 6845 keys, 32 heads of 64: 352 workgroups on
+        // 256 CUs, two cuts, 138 -> 118 us.
+        const double t1 = 4.0 * a->B * a->H * (double)a->Lq * a->Lk * pl.hd / 5e14, round1 = (double)((blocks + 255) / 256);
+        double best = t1;
+        for (int ns = 2; ns <= 4 && ns <= (tiles + 7) / 8; ++ns) {
+            const double t = t1 * (double)((blocks * ns + 255) / 256) / ns / round1 + 8.0 * ns * a->B * a->Hkv * R * pl.hdp / 4e12 + 5e-6;
+            if (t < 0.95 * best) { best = t; pl.ns = ns; }
+        }
     }
     pl.part_bytes = pl.ns > 1 ? (int64_t)pl.ns * a->B * a->Hkv * R * (pl.hdp + 2) * 4 : 0;
     return pl;
 }
 
-template <typename T, int HDP> int launch_fwd(const Fwd& f, bool few, hipStream_t s) {
+template <typename T, int HD> int launch_fwd(const Fwd& f, bool few, hipStream_t s) {
+    constexpr int HDP = padded(HD);
     const int64_t blocks = (int64_t)f.p.B * f.p.Hkv * f.nrb * f.ns;
     MARS_CHECK(blocks * 256 < (1ll << 32), "cross_attn: %lld workgroups are more than a launch takes", (long long)blocks);
     const dim3 grid((unsigned)blocks), block(256);
     if (f.p.bias != nullptr) {
-        if (few) hipLaunchKernelGGL((cross_fwd_kernel<T, HDP, true, true>), grid, block, 0, s, f);
-        else hipLaunchKernelGGL((cross_fwd_kernel<T, HDP, true, false>), grid, block, 0, s, f);
+        if (few) hipLaunchKernelGGL((cross_fwd_kernel<T, HD, true, true>), grid, block, 0, s, f);
+        else hipLaunchKernelGGL((cross_fwd_kernel<T, HD, true, false>), grid, block, 0, s, f);
     } else {
-        if (few) hipLaunchKernelGGL((cross_fwd_kernel<T, HDP, false, true>), grid, block, 0, s, f);
-        else hipLaunchKernelGGL((cross_fwd_kernel<T, HDP, false, false>), grid, block, 0, s, f);
+        if (few) hipLaunchKernelGGL((cross_fwd_kernel<T, HD, false, true>), grid, block, 0, s, f);
+        else hipLaunchKernelGGL((cross_fwd_kernel<T, HD, false, false>), grid, block, 0, s, f);
     }
     MARS_LAUNCH_CHECK();
     if (f.ns > 1) {
         const int64_t rows = (int64_t)f.p.B * f.p.Hkv * f.p.R;
-        MARS_CHECK((rows + 3) / 4 * 256 < (1ll << 32), "cross_attn: more workgroups than a launch takes");
-        hipLaunchKernelGGL((cross_join_kernel<T, HDP>), dim3((unsigned)((rows + 3) / 4)), block, 0, s, f);
+        const bool deep = f.ns > 4;
+        const int64_t per = deep ? 4 : 4 * (64 / (HDP / 4 == 24 ? 32 : HDP / 4)), groups = (rows + per - 1) / per;
+        MARS_CHECK(groups * 256 < (1ll << 32), "cross_attn: more workgroups than a launch takes");
+        if (deep) hipLaunchKernelGGL((cross_join_kernel<T, HDP, true>), dim3((unsigned)groups), block, 0, s, f);
+        else hipLaunchKernelGGL((cross_join_kernel<T, HDP, false>), dim3((unsigned)groups), block, 0, s, f);
         MARS_LAUNCH_CHECK();
     }
     return 0;
 }
 
 template <typename T> int launch_fwd_hd(const Fwd& f, const FwdPlan& pl, hipStream_t s) {
-    switch (pl.hdp) {
+    switch (pl.hd) {
+        case 16: return launch_fwd<T, 16>(f, pl.few, s);
         case 32: return launch_fwd<T, 32>(f, pl.few, s);
         case 64: return launch_fwd<T, 64>(f, pl.few, s);
+        case 80: return launch_fwd<T, 80>(f, pl.few, s);
         case 96: return launch_fwd<T, 96>(f, pl.few, s);
         default: return launch_fwd<T, 128>(f, pl.few, s);
     }

@@ -53,10 +53,11 @@ template <bool BIAS> __device__ __forceinline__ float prob(float s, float c2, fl
     return BIAS ? __builtin_amdgcn_exp2f((s - off) * LOG2E) * fac : __builtin_amdgcn_exp2f(fmaf(s, c2, -off));
 }
 
-template <typename T, int HDP, bool BIAS>
-__global__ __launch_bounds__(256, (q_waves<T, HDP, BIAS>())) void cross_bwd_q_kernel(const Bwd f) {
+template <typename T, int HD, bool BIAS>
+__global__ __launch_bounds__(256, (q_waves<T, padded(HD), BIAS>())) void cross_bwd_q_kernel(const Bwd f) {
+    constexpr int HDP = padded(HD);
     using TL = Tile<T, HDP>;
-    constexpr int KT = (HDP > 64 && sizeof(T) == 4) || q_waves<T, HDP, BIAS>() == 3 ? 32 : 64, TB = KT * TL::ROWB, KB = KT / 32, KS = HDP / 16, DM = HDP / 32;
+    constexpr int KT = (HDP > 64 && sizeof(T) == 4) || q_waves<T, HDP, BIAS>() == 3 ? 32 : 64, TB = KT * TL::ROWB, KB = KT / 32, KS = HD / 16, DM = HDP / 32;
     __shared__ __attribute__((aligned(16))) unsigned char buf0[2][TB];
     __shared__ __attribute__((aligned(16))) unsigned char buf1[2][TB];
     const Prob& p = f.p;
@@ -235,11 +236,12 @@ template <typename T, int HDP> struct KeyCfg {
     static constexpr int TB = QT * Tile<T, HDP>::ROWB, RB = QT / 32 * RSB * 4;
 };
 
-template <typename T, int HDP, bool BIAS>
-__global__ __launch_bounds__(256, (kv_waves<T, HDP>())) void cross_bwd_kv_kernel(const Bwd f) {
+template <typename T, int HD, bool BIAS>
+__global__ __launch_bounds__(256, (kv_waves<T, padded(HD)>())) void cross_bwd_kv_kernel(const Bwd f) {
+    constexpr int HDP = padded(HD);
     using TL = Tile<T, HDP>;
     using Cfg = KeyCfg<T, HDP>;
-    constexpr int QT = Cfg::QT, TB = Cfg::TB, KS = HDP / 16, DM = HDP / 32;
+    constexpr int QT = Cfg::QT, TB = Cfg::TB, KS = HD / 16, DM = HDP / 32;
     __shared__ __attribute__((aligned(16))) unsigned char buf0[2 * TB + Cfg::RB];
     __shared__ __attribute__((aligned(16))) unsigned char buf1[2 * TB + Cfg::RB];
     const Prob& p = f.p;
@@ -441,10 +443,11 @@ __global__ __launch_bounds__(256) void cross_bwd_sum_kernel(const Bwd f) {
 // dbias[h, i, j] = sum_b dS: grid (key tiles of 64, query blocks of 128, heads); keys are taken where they stand (the lists of attended keys
 // differ from entry to entry), with the key as lane column so that rows of bias and dbias are read and written in whole lines.  While one
 // batch entry is worked on, the next one's K and V tiles, query rows and row values are on their way.
-template <typename T, int HDP>
-__global__ __launch_bounds__(256, (HDP <= 64 && sizeof(T) == 2) ? 2 : 1) void cross_bwd_bias_kernel(const Bwd f) {
+template <typename T, int HD>
+__global__ __launch_bounds__(256, (HD <= 64 && sizeof(T) == 2) ? 2 : 1) void cross_bwd_bias_kernel(const Bwd f) {
+    constexpr int HDP = padded(HD);
     using TL = Tile<T, HDP>;
-    constexpr int KT = 64, TB = KT * TL::ROWB, KS = HDP / 16;
+    constexpr int KT = 64, TB = KT * TL::ROWB, KS = HD / 16;
     __shared__ __attribute__((aligned(16))) unsigned char buf0[2][TB];
     __shared__ __attribute__((aligned(16))) unsigned char buf1[2][TB];
     __shared__ __attribute__((aligned(16))) float rowv[4][3][32];
@@ -545,7 +548,7 @@ __global__ __launch_bounds__(256, (HDP <= 64 && sizeof(T) == 2) ? 2 : 1) void cr
         }
 }
 
-struct BwdPlan { int hdp, nrb, nsq, nkb, nsk; int64_t rows_bytes, q_bytes, e_bytes, k_bytes; };
+struct BwdPlan { int hd, hdp, nrb, nsq, nkb, nsk; int64_t rows_bytes, q_bytes, e_bytes, k_bytes; };
 int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
 
 int splits(int64_t blocks, int64_t most) {
@@ -558,7 +561,8 @@ int splits(int64_t blocks, int64_t most) {
 BwdPlan plan_bwd(const MarsCrossAttn* a) {
     BwdPlan pl;
     const int64_t R = (int64_t)(a->H / a->Hkv) * a->Lq, nbh = (int64_t)a->B * a->Hkv;
-    pl.hdp = (a->hd + 31) / 32 * 32;
+    pl.hd = built_for(a->hd);
+    pl.hdp = padded(pl.hd);
     pl.nrb = (int)((R + 127) / 128);
     pl.nkb = (a->Lk + 127) / 128;
     pl.nsq = splits(nbh * pl.nrb, ((int64_t)a->Lk + 127) / 128);
@@ -570,20 +574,21 @@ BwdPlan plan_bwd(const MarsCrossAttn* a) {
     return pl;
 }
 
-template <typename T, int HDP> int launch_bwd(const Bwd& f, hipStream_t s) {
+template <typename T, int HD> int launch_bwd(const Bwd& f, hipStream_t s) {
+    constexpr int HDP = padded(HD);
     const Prob& p = f.p;
     const int64_t nbh = (int64_t)p.B * p.Hkv, qb = nbh * f.nrb * f.nsq, kb = nbh * f.nkb * f.nsk, per = 256 / (HDP / 4);
     MARS_CHECK(qb * 256 < (1ll << 32) && kb * 256 < (1ll << 32), "cross_attn_bwd: more workgroups than a launch takes");
     const dim3 block(256);
-    if (p.bias != nullptr) hipLaunchKernelGGL((cross_bwd_q_kernel<T, HDP, true>), dim3((unsigned)qb), block, 0, s, f);
-    else hipLaunchKernelGGL((cross_bwd_q_kernel<T, HDP, false>), dim3((unsigned)qb), block, 0, s, f);
+    if (p.bias != nullptr) hipLaunchKernelGGL((cross_bwd_q_kernel<T, HD, true>), dim3((unsigned)qb), block, 0, s, f);
+    else hipLaunchKernelGGL((cross_bwd_q_kernel<T, HD, false>), dim3((unsigned)qb), block, 0, s, f);
     MARS_LAUNCH_CHECK();
     if (f.nsq > 1) {
         hipLaunchKernelGGL((cross_bwd_sum_kernel<T, HDP, false>), dim3((unsigned)((nbh * p.R + per - 1) / per)), block, 0, s, f);
         MARS_LAUNCH_CHECK();
     }
-    if (p.bias != nullptr) hipLaunchKernelGGL((cross_bwd_kv_kernel<T, HDP, true>), dim3((unsigned)kb), block, 0, s, f);
-    else hipLaunchKernelGGL((cross_bwd_kv_kernel<T, HDP, false>), dim3((unsigned)kb), block, 0, s, f);
+    if (p.bias != nullptr) hipLaunchKernelGGL((cross_bwd_kv_kernel<T, HD, true>), dim3((unsigned)kb), block, 0, s, f);
+    else hipLaunchKernelGGL((cross_bwd_kv_kernel<T, HD, false>), dim3((unsigned)kb), block, 0, s, f);
     MARS_LAUNCH_CHECK();
     if (f.nsk > 1) {
         hipLaunchKernelGGL((cross_bwd_sum_kernel<T, HDP, true>), dim3((unsigned)((nbh * p.Lk + per - 1) / per), 2), block, 0, s, f);
@@ -592,16 +597,18 @@ template <typename T, int HDP> int launch_bwd(const Bwd& f, hipStream_t s) {
     if (f.dbias != nullptr) {
         const unsigned gy = (unsigned)((p.Lq + 127) / 128);
         MARS_CHECK(gy <= 65535 && p.H <= 65535, "cross_attn_bwd: more workgroups than a launch takes");
-        hipLaunchKernelGGL((cross_bwd_bias_kernel<T, HDP>), dim3((unsigned)((p.Lk + 63) / 64), gy, (unsigned)p.H), block, 0, s, f);
+        hipLaunchKernelGGL((cross_bwd_bias_kernel<T, HD>), dim3((unsigned)((p.Lk + 63) / 64), gy, (unsigned)p.H), block, 0, s, f);
         MARS_LAUNCH_CHECK();
     }
     return 0;
 }
 
-template <typename T> int launch_bwd_hd(const Bwd& f, int hdp, hipStream_t s) {
-    switch (hdp) {
+template <typename T> int launch_bwd_hd(const Bwd& f, int hd, hipStream_t s) {
+    switch (hd) {
+        case 16: return launch_bwd<T, 16>(f, s);
         case 32: return launch_bwd<T, 32>(f, s);
         case 64: return launch_bwd<T, 64>(f, s);
+        case 80: return launch_bwd<T, 80>(f, s);
         case 96: return launch_bwd<T, 96>(f, s);
         default: return launch_bwd<T, 128>(f, s);
     }
@@ -641,5 +648,5 @@ extern "C" int marship_cross_attn_bwd(const MarsCrossAttn* a, void* stream) {
     f.mask = a->mask;
     f.kv_len = a->kv_len;
     f.nrb = pl.nrb; f.nsq = pl.nsq; f.nkb = pl.nkb; f.nsk = pl.nsk;
-    return a->dtype == 1 ? launch_bwd_hd<__bf16>(f, pl.hdp, s) : launch_bwd_hd<float>(f, pl.hdp, s);
+    return a->dtype == 1 ? launch_bwd_hd<__bf16>(f, pl.hd, s) : launch_bwd_hd<float>(f, pl.hd, s);
 }
