@@ -13,6 +13,7 @@
 //   keys     a wave owns 32 keys and walks the query rows of every head that shares them: S = Q K^T, dP = dO V^T with the key as
 //            lane column; P and dS are the operands of dV^T += dO^T P and dK^T += Q^T dS.
 //   bias     (only where its gradient is asked for) a wave owns a 32 x 64 piece of one head's scores and walks the batch.
+// With one attended key P is 1 whatever the score and dS is 0: dQ, dK and dbias are set to it, because dP - D is the difference of two roundings of one number.
 // Recomputing S and dP in each pass costs 2 of 7 products more than one pass over all would, but that one would add into dQ from
 // every key block: atomics, in an order that changes.
 #include <type_traits>
@@ -200,6 +201,7 @@ __global__ __launch_bounds__(256, (q_waves<T, padded(HD), BIAS>())) void cross_b
         rs[64] = f.nsq > 1 ? D : D + e;
     }
     if (!row_ok) return;
+    const bool one = n <= 1;
     if (f.nsq > 1) {
         const int64_t row = ((int64_t)split * p.B * p.Hkv + bh) * p.R + r;
         float* po = f.part_q + row * HDP * (MEND ? 2 : 1);
@@ -208,10 +210,10 @@ __global__ __launch_bounds__(256, (q_waves<T, padded(HD), BIAS>())) void cross_b
 #pragma unroll
             for (int a = 0; a < 4; ++a) {
                 const int d = 32 * m + 8 * a + 4 * hh;
-                *(f32x4*)(po + d) = (f32x4){dq[m][4 * a], dq[m][4 * a + 1], dq[m][4 * a + 2], dq[m][4 * a + 3]};
+                *(f32x4*)(po + d) = (f32x4){one ? 0.f : dq[m][4 * a], one ? 0.f : dq[m][4 * a + 1], one ? 0.f : dq[m][4 * a + 2], one ? 0.f : dq[m][4 * a + 3]};
                 if constexpr (MEND) *(f32x4*)(po + HDP + d) = (f32x4){pk[m][4 * a], pk[m][4 * a + 1], pk[m][4 * a + 2], pk[m][4 * a + 3]};
             }
-        if (MEND && hh == 0) f.part_e[row] = e;
+        if (MEND && hh == 0) f.part_e[row] = one ? 0.f : e;
         return;
     }
     T* out = (T*)f.dq + b * f.sdq.b + l * f.sdq.l + h * f.sdq.h;
@@ -225,7 +227,7 @@ __global__ __launch_bounds__(256, (q_waves<T, padded(HD), BIAS>())) void cross_b
             for (int c = 0; c < 4; ++c) {
                 v[c] = dq[m][4 * a + c];
                 if constexpr (MEND) v[c] = fmaf(-e, pk[m][4 * a + c], v[c]);
-                v[c] *= p.scale;
+                v[c] = one ? 0.f : v[c] * p.scale;
             }
             if (d < p.hd) store4(out + d, v[0], v[1], v[2], v[3]);
         }
@@ -360,6 +362,10 @@ __global__ __launch_bounds__(256, (kv_waves<T, padded(HD)>())) void cross_bwd_kv
         }
     }
     if (!exists) return;
+    if (n <= 1) {
+#pragma unroll
+        for (int m = 0; m < DM; ++m) dk[m] = zero16();
+    }
     if (f.nsk > 1) {
         const int64_t o = (((int64_t)split * p.B * p.Hkv + bh) * p.Lk + pos) * HDP;
 #pragma unroll
@@ -468,9 +474,9 @@ __global__ __launch_bounds__(256, (HD <= 64 && sizeof(T) == 2) ? 2 : 1) void cro
             bias[kb][i] = p.bias[h * p.bias_h + li * p.bias_l + j];
         }
     auto length = [&](int b) { return f.kv_len == nullptr ? p.Lk : min(max(f.kv_len[b], 0), p.Lk); };
-    // the next batch entry from b with keys in this tile (the same for the whole workgroup)
+    // the next batch entry from b with keys in this tile, and more than one in all (the same for the whole workgroup)
     auto entry = [&](int b) {
-        while (b < p.B && j0 >= length(b)) ++b;
+        while (b < p.B && (j0 >= length(b) || key_count(p, b) <= 1)) ++b;
         return b;
     };
     frag_t<T> qf[KS], dof[KS];

@@ -361,6 +361,7 @@ __global__ __launch_bounds__(TH) void norm_bwd_apply_kernel(const Norm a, const 
     const TX* xp = (const TX*)a.x + (int64_t)n * a.x_n + c;
     const TY* yp = (const TY*)d.dy + (int64_t)n * d.dy_n + c;
     TX* op = (TX*)d.dx + (int64_t)n * d.dx_n + c;
+    const bool one = a.P == 1 && a.Cg == 1;                         // a group of one value is its own mean: no gradient
     const int r1 = min((chunk + 1) * a.rows, a.P);
     for (int r = chunk * a.rows + rl; r < r1; r += nrl * KR) {
         float x[KR][V], y[KR][V];
@@ -377,7 +378,7 @@ __global__ __launch_bounds__(TH) void norm_bwd_apply_kernel(const Norm a, const 
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
                     const float xh = (x[k][e] - mean) * rstd, dz = y[k][e] * slope_of(fmaf(xh, w[e], b[e]), a.act);
-                    o[e] = rstd * (dz * w[e] - m1 - xh * m2);
+                    o[e] = one ? 0.f : rstd * (dz * w[e] - m1 - xh * m2);
                 }
                 store_vec<TX, V, STREAM>(op + (int64_t)(r + k * nrl) * d.dx_p, o);
             }
@@ -541,6 +542,7 @@ __global__ __launch_bounds__(TF) void norm_group_bwd_kernel(const Norm a, const 
     }
     if (!on) return;
     TX* op = (TX*)d.dx + (int64_t)n * d.dx_n + c;
+    const bool one = a.P == 1 && a.Cg == 1;                         // a group of one value is its own mean: no gradient
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         const int r = rl + k * step;
@@ -551,7 +553,7 @@ __global__ __launch_bounds__(TF) void norm_group_bwd_kernel(const Norm a, const 
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 const float xh = (xv[e] - mean) * rstd, dz = yv[e] * slope_of(fmaf(xh, w[e], b[e]), a.act);
-                xv[e] = rstd * (dz * w[e] - m1 - xh * m2);
+                xv[e] = one ? 0.f : rstd * (dz * w[e] - m1 - xh * m2);
             }
             store_vec<TX, V>(op + (int64_t)r * d.dx_p, xv);
         }

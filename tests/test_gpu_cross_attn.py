@@ -215,6 +215,25 @@ def test_masks(pkg, cuda, dtype, keys, Lq):
 
 
 @pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("Lq,Lk,how,bias", [(9, 1, "all", "rand"), (200, 1, "all", None), (40, 70, "len", "rand"), (150, 300, "mask", None), (3, 3000, "mask", "rand")])
+def test_one_attended_key_has_no_gradient_of_scores(pkg, cuda, dtype, Lq, Lk, how, bias):
+    """the softmax over one key is 1: q, k and the bias have a gradient of exactly zero"""
+    c = make(cuda, dtype, 2, Lq, Lk, 4, 2, 64, seed=13, bias=bias)
+    att = torch.zeros(2, Lk, dtype=torch.bool)
+    att[:, 0 if how == "len" else Lk // 2] = True
+    c["att"] = att
+    if how == "len":
+        c["kv_len"] = torch.ones(2, dtype=torch.int32, device=cuda)
+    if how == "mask":
+        c["mask"] = att.to(cuda)
+    got = run(pkg, c)
+    for n in ("dq", "dk", "dbias"):
+        assert got[n] is None or bool((got[n] == 0).all()), n
+    res, tol = reference(c)
+    assert bool(((got["dv"].double() - res["dv"]).abs() <= tol["dv"]).all()) and bool(((got["out"].double() - res["out"]).abs() <= tol["out"]).all())
+
+
+@pytest.mark.parametrize("dtype", DT)
 @pytest.mark.parametrize("bias", ["rand", "inf", "low"])
 @pytest.mark.parametrize("Lq,Lk,keys", [(6, 90, "all"), (150, 131, "mask"), (40, 700, "len")])
 def test_bias(pkg, cuda, dtype, bias, Lq, Lk, keys):

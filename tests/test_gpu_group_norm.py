@@ -156,6 +156,15 @@ def test_constant_group_and_nan(pkg, cuda):
     assert bool(torch.isnan(out[0, :, :8]).all()) and bool((out[0, :, 8:] == 0.25).all()) and bool((out[1] == 0.25).all())
 
 
+def test_groups_of_one_value_have_no_gradient(pkg, cuda):
+    x, dy, w, b = (torch.randn(*s, device=cuda) for s in ((3, 1, 24), (3, 1, 24), (24,), (24,)))
+    stat, out, dx, dw, db = (torch.empty(*s, device=cuda) for s in ((3, 24, 2), (3, 1, 24), (3, 1, 24), (24,), (24,)))
+    pkg.ops.group_norm_act(x, w, b, out, 24, EPS, 4, stat=stat)
+    assert torch.equal(stat[..., 0], x[:, 0])
+    pkg.ops.group_norm_act_bwd(x, w, b, stat, dy, dx, dw, db, 24, 4)
+    assert bool((dx == 0).all()) and bool((dw == 0).all())
+
+
 @pytest.mark.parametrize("act", [0, 1, 2, 4])
 def test_gradients_against_differences(pkg, cuda, act):
     """<gradient, direction> against central differences of the definition in 64 bits (step 1e-4: off by about 1e-8 of the magnitudes)"""
