@@ -11,6 +11,11 @@
 // batch entry, and the fills gather K and V rows through that list.  A support image's foreground is a tenth to
 // a half of its patches, a row costs the same gathered or not (it is at least one 32-byte sector, mostly one or two cache lines),
 // and whatever stands in a masked row - infinities, NaN - is never read.
+//
+// Few rows (one new token a sequence) are bound by memory: the four waves of a workgroup take key tiles in turn through buffers of their own, the keys
+// are cut over the chip and joined (16 sequences over up to 8192 keys, 16 / 4 heads of 128: 40 us for 206 MB).  Many rows are bound by
+// vector ALU: a score costs 16 cycles of exponential and 14 of other work against 8 (64-wide heads) of matrix instructions;
+// 1369 over 6845, 32 heads of 64: 116 us with the join of two cuts, 660 TFLOP/s.
 #include <type_traits>
 #include "attention_cross.h"
 

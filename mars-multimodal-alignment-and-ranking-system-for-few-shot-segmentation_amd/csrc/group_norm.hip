@@ -7,6 +7,8 @@
 // Bound by memory: a thread owns V neighbouring channels (16 bytes of bf16) of every few rows, so a wave reads and writes whole
 // lines, and keeps the channels' parameters in registers.  A map is cut into chunks of rows; the chunks' statistics
 // (count, mean, sum of squares about the mean - no difference of large sums) are joined in a small launch, always in the same order.
+// 16 maps of 128 x 128 x 256 bf16: 22 us statistics, 5 join, 47 result.  Where a workgroup can hold a group, and its piece of a row is 64 bytes or more, one
+// launch does it all (1369 x 1024, 32 groups: 10 us against 17 in three; pieces of 16 bytes: 99 against 77).
 #include <initializer_list>
 #include "common.h"
 #include "../../include/mars_hip.h"
