@@ -31,6 +31,7 @@ namespace {
 // and factor = 1 / sum: where the mask is the type's lowest value the sum's logarithm would be lost in the maximum.
 // Rows that do not exist or have no key: P = 0.
 constexpr int RSB = 128;
+constexpr int FEW_KEYS = 256;           // see cross_bwd_q_kernel
 // waves a SIMD that the two passes are built for (three of the key pass's would spill: 109 -> 142 us on eight 1369 x 684 x 16 heads of 64; the query
 // pass with three, walking tiles of 32 keys: 98 -> 89)
 template <typename T, int HDP, bool BIAS> constexpr int q_waves() { return sizeof(T) == 4 || HDP > 96 ? 1 : HDP > 64 || BIAS ? 2 : 3; }
@@ -55,11 +56,14 @@ template <bool BIAS> __device__ __forceinline__ float prob(float s, float c2, fl
     return BIAS ? __builtin_amdgcn_exp2f((s - off) * LOG2E) * fac : __builtin_amdgcn_exp2f(fmaf(s, c2, -off));
 }
 
-template <typename T, int HD, bool BIAS>
-__global__ __launch_bounds__(256, (q_waves<T, padded(HD), BIAS>())) void cross_bwd_q_kernel(const Bwd f) {
+// FINE (bf16, up to FEW_KEYS keys): what the rounding of dS leaves over goes through the matrix instruction too, and dQ is off by its own rounding alone (1.7e-3
+// in norm; 2.4e-3 with a rounded dS, up to 2.6e-3 where the keys are few).  A fifth product: nothing where the launch is the time, a fifth
+// of this pass on long axes, where it is left out as it is for dK and dV.
+template <typename T, int HD, bool BIAS, bool FINE>
+__global__ __launch_bounds__(256, (q_waves<T, padded(HD), BIAS || FINE>())) void cross_bwd_q_kernel(const Bwd f) {
     constexpr int HDP = padded(HD);
     using TL = Tile<T, HDP>;
-    constexpr int KT = (HDP > 64 && sizeof(T) == 4) || q_waves<T, HDP, BIAS>() == 3 ? 32 : 64, TB = KT * TL::ROWB, KB = KT / 32, KS = HD / 16, DM = HDP / 32;
+    constexpr int KT = (HDP > 64 && sizeof(T) == 4) || q_waves<T, HDP, BIAS || FINE>() == 3 ? 32 : 64, TB = KT * TL::ROWB, KB = KT / 32, KS = HD / 16, DM = HDP / 32;
     __shared__ __attribute__((aligned(16))) unsigned char buf0[2][TB];
     __shared__ __attribute__((aligned(16))) unsigned char buf1[2][TB];
     const Prob& p = f.p;
@@ -162,12 +166,17 @@ __global__ __launch_bounds__(256, (q_waves<T, padded(HD), BIAS>())) void cross_b
             for (int u = 0; u < 2; ++u) {
                 // (dS of bf16 heads is rounded to bf16 for the matrix instruction, as P is in the forward pass)
                 const frag_t<T> df = pack_step<T>(dp, u);
-                frag_t<T> pf = df;
+                frag_t<T> pf = df, rest = df;
                 if constexpr (MEND) pf = pack_step<T>(s, u);
+                if constexpr (FINE) {
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) rest[x] = (T)(dp[8 * u + x] - (float)df[x]);
+                }
 #pragma unroll
                 for (int m = 0; m < DM; ++m) {
                     const frag_t<T> kc = TL::cols(kt, 32 * kb + 16 * u, m, lane);
                     dq[m] = mma(kc, df, dq[m]);
+                    if constexpr (FINE) dq[m] = mma(kc, rest, dq[m]);
                     if constexpr (MEND) pk[m] = mma(kc, pf, pk[m]);
                 }
             }
@@ -587,8 +596,14 @@ template <typename T, int HD> int launch_bwd(const Bwd& f, hipStream_t s) {
     const int64_t nbh = (int64_t)p.B * p.Hkv, qb = nbh * f.nrb * f.nsq, kb = nbh * f.nkb * f.nsk, per = 256 / (HDP / 4);
     MARS_CHECK(qb * 256 < (1ll << 32) && kb * 256 < (1ll << 32), "cross_attn_bwd: more workgroups than a launch takes");
     const dim3 block(256);
-    if (p.bias != nullptr) hipLaunchKernelGGL((cross_bwd_q_kernel<T, HD, true>), dim3((unsigned)qb), block, 0, s, f);
-    else hipLaunchKernelGGL((cross_bwd_q_kernel<T, HD, false>), dim3((unsigned)qb), block, 0, s, f);
+    constexpr bool F = sizeof(T) == 2;
+    if (p.Lk <= FEW_KEYS) {
+        if (p.bias != nullptr) hipLaunchKernelGGL((cross_bwd_q_kernel<T, HD, true, F>), dim3((unsigned)qb), block, 0, s, f);
+        else hipLaunchKernelGGL((cross_bwd_q_kernel<T, HD, false, F>), dim3((unsigned)qb), block, 0, s, f);
+    } else {
+        if (p.bias != nullptr) hipLaunchKernelGGL((cross_bwd_q_kernel<T, HD, true, false>), dim3((unsigned)qb), block, 0, s, f);
+        else hipLaunchKernelGGL((cross_bwd_q_kernel<T, HD, false, false>), dim3((unsigned)qb), block, 0, s, f);
+    }
     MARS_LAUNCH_CHECK();
     if (f.nsq > 1) {
         hipLaunchKernelGGL((cross_bwd_sum_kernel<T, HDP, false>), dim3((unsigned)((nbh * p.R + per - 1) / per)), block, 0, s, f);
