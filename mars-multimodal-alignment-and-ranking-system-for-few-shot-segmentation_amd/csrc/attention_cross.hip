@@ -197,8 +197,8 @@ __global__ __launch_bounds__(256, (FwdCfg<T, HD, FEW>::WPE)) void cross_fwd_kern
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                // probabilities of bf16 heads are rounded to bf16 for the matrix instruction (half a step, 2^-9 of each, with signs
-                // that do not agree: far below the rounding of the result); their sum is taken before the rounding
+                // probabilities of bf16 heads are rounded to bf16 for the matrix instruction (at most half a step, 2^-8 of each, with signs
+                // that do not agree: below the rounding of the result); their sum is taken before the rounding
                 const frag_t<T> pf = pack_step<T>(s[kb], u);
 #pragma unroll
                 for (int m = 0; m < DM; ++m) o[m] = mma(TL::cols(vt, 32 * kb + 16 * u, m, lane), pf, o[m]);
@@ -528,6 +528,7 @@ int64_t key_ws_bytes(const MarsCrossAttn* a) { return a->mask ? align256((int64_
 
 int prepare_keys(const MarsCrossAttn* a, Prob& p, int32_t* ws, hipStream_t s) {
     if (a->mask == nullptr) return 0;
+    MARS_CHECK((int64_t)a->B * 1024 < (1ll << 32), "cross_attn: %d batch entries are more than a launch takes", a->B);
     int32_t* cnt = (int32_t*)((char*)ws + align256((int64_t)a->B * a->Lk * 4));
     hipLaunchKernelGGL(list_keys_kernel, dim3((unsigned)a->B), dim3(1024), 0, s, a->mask, a->kv_len, a->Lk, ws, cnt);
     MARS_LAUNCH_CHECK();
