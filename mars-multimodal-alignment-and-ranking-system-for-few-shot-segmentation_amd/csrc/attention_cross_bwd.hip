@@ -29,7 +29,8 @@ namespace {
 // Row values of 32 query rows: 128 floats - [0, 32) offset of the exponent, [32, 64) factor of the exponential (bias only), [64, 96) D.
 // Without a bias P = 2^(c2 s - offset) with offset = log2(e) maximum + log2(sum).  With one, P = 2^((s - offset) log2 e) factor with offset = maximum
 // and factor = 1 / sum: where the mask is the type's lowest value the sum's logarithm would be lost in the maximum.
-// Rows that do not exist or have no key: P = 0.
+// Rows that do not exist or have no key: offset +inf and factor 0, so that the exponential itself is 0 whatever the score.  (The key pass holds the last row
+// again in their place: with an offset of 0 a score above 88.7 of it would be inf * 0.)
 constexpr int RSB = 128;
 constexpr int FEW_KEYS = 256;           // see cross_bwd_q_kernel
 // waves a SIMD that the two passes are built for (three of the key pass's would spill: 109 -> 142 us on eight 1369 x 684 x 16 heads of 64; the query
@@ -110,7 +111,7 @@ __global__ __launch_bounds__(256, (q_waves<T, padded(HD), BIAS || FINE>())) void
     const T* dorow = row_ok ? row_ptr<T>(p.dout, p.sdo, b, l, h) : nullptr;
     const T* orow = row_ok ? row_ptr<T>(p.out, p.so, b, l, h) : nullptr;
     const float c2 = p.scale * LOG2E;
-    float D = 0.f, off = BIAS ? 0.f : INFINITY, fac = 0.f;
+    float D = 0.f, off = INFINITY, fac = 0.f;
     if (row_ok) {
         const float* st = p.stat + (((int64_t)b * p.H + h) * p.Lq + l) * 2;
         const float m = st[0], sum = st[1];
