@@ -50,6 +50,7 @@ struct Bwd {
     float *part_q, *part_k, *part_v; // [ns][..][HDP] partial sums, where a pass is split (part_q bf16: dS' K, then P K, of a row)
     float* part_e;                   // [nsq][B Hkv][R]: partial sums of dS'
     int nrb, nsq;                    // query pass: blocks of 128 rows, splits of the keys
+    int by_count;                    // query pass: two launches, for entries of up to FEW_KEYS attended keys and for the others
     int nkb, nsk;                    // key pass: blocks of 128 keys, splits of the query rows
 };
 
@@ -57,9 +58,10 @@ template <bool BIAS> __device__ __forceinline__ float prob(float s, float c2, fl
     return BIAS ? __builtin_amdgcn_exp2f((s - off) * LOG2E) * fac : __builtin_amdgcn_exp2f(fmaf(s, c2, -off));
 }
 
-// FINE (bf16, up to FEW_KEYS keys): what the rounding of dS leaves over goes through the matrix instruction too, and dQ is off by its own rounding alone (1.7e-3
-// in norm; 2.4e-3 with a rounded dS, up to 2.6e-3 where the keys are few).  A fifth product: nothing where the launch is the time, a fifth
-// of this pass on long axes, where it is left out as it is for dK and dV.
+// FINE (bf16, up to FEW_KEYS attended keys): what the rounding of dS leaves over goes through the matrix instruction too, and dQ is off by its own rounding alone
+// (1.7e-3 in norm; 2.4e-3 with a rounded dS, up to 2.6e-3 where the keys are few).  A fifth product: nothing where the launch is the time, a fifth
+// of this pass on long axes, where it is left out as it is for dK and dV.  How many keys of a long axis an entry attends to is known on the device alone:
+// there both forms are launched and each takes its own entries (one kernel with both loops would need the registers of both).
 template <typename T, int HD, bool BIAS, bool FINE>
 __global__ __launch_bounds__(256, (q_waves<T, padded(HD), BIAS || FINE>())) void cross_bwd_q_kernel(const Bwd f) {
     constexpr int HDP = padded(HD);
@@ -79,6 +81,7 @@ __global__ __launch_bounds__(256, (q_waves<T, padded(HD), BIAS || FINE>())) void
     int l = 0, h = 0;
     if (row_ok) row_of(p, hk, r, l, h);
     const int n = key_count(p, b);
+    if (f.by_count && (n <= FEW_KEYS) != FINE) return;              // (the whole workgroup)
     const int32_t* idx = p.idx == nullptr ? nullptr : p.idx + (int64_t)b * p.Lk;
     const int hdb = p.hd * (int)sizeof(T);
     const unsigned char* kbase = (const unsigned char*)row_ptr<T>(p.k, p.sk, b, 0, hk);
@@ -598,14 +601,19 @@ template <typename T, int HD> int launch_bwd(const Bwd& f, hipStream_t s) {
     MARS_CHECK(qb * 256 < (1ll << 32) && kb * 256 < (1ll << 32), "cross_attn_bwd: more workgroups than a launch takes");
     const dim3 block(256);
     constexpr bool F = sizeof(T) == 2;
-    if (p.Lk <= FEW_KEYS) {
-        if (p.bias != nullptr) hipLaunchKernelGGL((cross_bwd_q_kernel<T, HD, true, F>), dim3((unsigned)qb), block, 0, s, f);
-        else hipLaunchKernelGGL((cross_bwd_q_kernel<T, HD, false, F>), dim3((unsigned)qb), block, 0, s, f);
-    } else {
-        if (p.bias != nullptr) hipLaunchKernelGGL((cross_bwd_q_kernel<T, HD, true, false>), dim3((unsigned)qb), block, 0, s, f);
-        else hipLaunchKernelGGL((cross_bwd_q_kernel<T, HD, false, false>), dim3((unsigned)qb), block, 0, s, f);
+    const bool few = F && p.Lk <= FEW_KEYS, both = F && !few && p.cnt != nullptr;
+    Bwd fq = f;
+    fq.by_count = both;
+    if (few || both) {
+        if (p.bias != nullptr) hipLaunchKernelGGL((cross_bwd_q_kernel<T, HD, true, F>), dim3((unsigned)qb), block, 0, s, fq);
+        else hipLaunchKernelGGL((cross_bwd_q_kernel<T, HD, false, F>), dim3((unsigned)qb), block, 0, s, fq);
+        MARS_LAUNCH_CHECK();
     }
-    MARS_LAUNCH_CHECK();
+    if (!few) {
+        if (p.bias != nullptr) hipLaunchKernelGGL((cross_bwd_q_kernel<T, HD, true, false>), dim3((unsigned)qb), block, 0, s, fq);
+        else hipLaunchKernelGGL((cross_bwd_q_kernel<T, HD, false, false>), dim3((unsigned)qb), block, 0, s, fq);
+        MARS_LAUNCH_CHECK();
+    }
     if (f.nsq > 1) {
         hipLaunchKernelGGL((cross_bwd_sum_kernel<T, HDP, false>), dim3((unsigned)((nbh * p.R + per - 1) / per)), block, 0, s, f);
         MARS_LAUNCH_CHECK();

@@ -1,8 +1,8 @@
-"""Attention between two token sets where it once went wrong, or could: very large scores with a bias."""
+"""Attention between two token sets where it once went wrong, or could: very large scores with a bias, a few attended keys of a long axis."""
 import pytest
 import torch
 
-from tests.test_gpu_cross_attn import DT, check, make
+from tests.test_gpu_cross_attn import DT, U32, check, make, run
 
 pytestmark = pytest.mark.gpu
 
@@ -19,3 +19,44 @@ def test_gradients_of_large_scores(pkg, cuda, dtype, bias, Lq, keys):
     last = c["q"][0, -1, 1].float() @ c["k"][0, on, 0].float().t() * c["scale"]        # (rows of heads 0 and 1 are one list: the last is head 1's)
     assert float(last.max()) > 100
     check(pkg, c)
+
+
+@pytest.mark.parametrize("how", ["mask", "len"])
+@pytest.mark.parametrize("bias", [None, "rand"])
+@pytest.mark.parametrize("hd", [16, 64, 80, 128])
+def test_masked_keys_and_absent_keys_give_the_same_gradient(pkg, cuda, how, bias, hd):
+    """dQ over the attended keys of a long axis against dQ over those keys alone, bf16: the same precision however the keys are left out.
+
+    Both calls multiply the same numbers and differ in the order of f32 sums over n keys: by at most c U32 M for a sum of magnitudes M, with c = n + 8 for each of
+    them, on a value x before its rounding to bf16.  A rounding turns that into a whole step (at most 2^-7 |x|) with probability c U32 M / step and into
+    nothing otherwise, so the squares of the differences add up to about sum c U32 M 2^-7 |x|; four times that for the spread of a count of flips."""
+    counts = [70, 256, 257, 300]
+    c = make(cuda, torch.bfloat16, 4, 150, 1369, 2, 2, hd, seed=hd, bias=bias)
+    g = torch.Generator().manual_seed(hd)
+    att = torch.zeros(4, 1369, dtype=torch.bool)
+    for b, n in enumerate(counts):
+        att[b, torch.randperm(1369, generator=g)[:n] if how == "mask" else torch.arange(n)] = True
+    c["att"] = att
+    if how == "mask":
+        c["mask"] = att.to(cuda)
+    else:
+        c["kv_len"] = torch.tensor(counts, dtype=torch.int32, device=cuda)
+    got = run(pkg, c)["dq"]
+    for b, n in enumerate(counts):
+        keys = torch.nonzero(att[b]).flatten().to(cuda)
+        one = dict(c, B=1, Lk=n, att=torch.ones(1, n, dtype=torch.bool), mask=None, kv_len=None, k=c["k"][b:b + 1, keys].contiguous(), v=c["v"][b:b + 1, keys].contiguous(),
+                   bias=None if bias is None else c["bias"][:, :, keys].contiguous())
+        for x in ("q", "dout"):
+            one[x] = c[x][b:b + 1].contiguous()
+        want = run(pkg, one)["dq"][0].double()
+        bound = 0.0
+        for h in range(2):
+            Q, K, V, dO = (one[x][0, :, h].double() for x in ("q", "k", "v", "dout"))
+            S = Q @ K.t() * c["scale"] + (0.0 if bias is None else one["bias"][h].double())
+            P = torch.softmax(S, 1)
+            D = (dO * (P @ V)).sum(1, keepdim=True)
+            dS = (P * (dO @ V.t() - D)).abs() + P * 2.0 ** -8 * (dO.abs() * (P @ V).abs()).sum(1, keepdim=True)      # (dS' with D from a rounded O)
+            M = c["scale"] * (dS @ K.abs() + dS.sum(1, keepdim=True) * (P @ K.abs()))
+            bound += float((2 * (n + 8) * U32 * M * 2.0 ** -7 * want[:, h].abs()).sum())
+        diff = float((got[b].double() - want).square().sum())
+        assert diff <= 4 * bound, f"{n} keys: {(diff / float(want.square().sum())) ** 0.5:.2e} of the norm, bound {(4 * bound / float(want.square().sum())) ** 0.5:.2e}"
