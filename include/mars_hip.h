@@ -184,7 +184,7 @@ int marship_flash_attn_mean(const void* qkv, const float* lse, int T, int H, int
  * Backward: dq, dk, dv (dk, dv: zeros at keys not attended) and, where dbias is not NULL, dbias f32 [H, Lq, Lk] by dbias_s, summed over the
  * batch.  Sums have a fixed order: results do not change from call to call.
  * ws: workspace of at least marship_cross_attn_ws(args, backward) bytes, 16-byte aligned, of the caller's and not shared
- * with a call that may run at the same time (it may be NULL where that is 0). */
+ * with a call that may run at the same time (it may be NULL where that is 0; a shape that the call refuses has 0 too). */
 typedef struct {
     const void *q, *k, *v;
     void* out;

@@ -485,17 +485,24 @@ static bool rows_ok(const void* ptr, const int64_t* st, int es) {
     return ((uintptr_t)ptr % 16 == 0) && (st[0] * es) % 16 == 0 && (st[1] * es) % 16 == 0 && (st[2] * es) % 16 == 0;
 }
 
+// what the workspace queries ask too: they divide by the counts of what a shape is cut into, and answer 0 for a shape that the call refuses
+static int check_shape(const MarsCrossAttn* a, const char* what) {
+    MARS_CHECK(a->B > 0 && a->Lq > 0 && a->Lk > 0 && a->H > 0 && a->Hkv > 0, "%s: bad shape B=%d Lq=%d Lk=%d H=%d Hkv=%d", what, a->B, a->Lq, a->Lk,
+               a->H, a->Hkv);
+    MARS_CHECK(a->H % a->Hkv == 0, "%s: %d query heads are no multiple of %d key heads", what, a->H, a->Hkv);
+    MARS_CHECK(a->hd > 0 && a->hd <= 128, "%s: head dim %d (up to 128, a multiple of 16 bytes)", what, a->hd);
+    MARS_CHECK((int64_t)(a->H / a->Hkv) * a->Lq < (1ll << 30) && a->Lk < (1 << 30), "%s: too many rows", what);
+    MARS_CHECK((int64_t)a->B * a->H < (1ll << 30), "%s: too many heads", what);
+    return 0;
+}
+
 int check(const MarsCrossAttn* a, bool backward) {
     const char* what = backward ? "cross_attn_bwd" : "cross_attn";
     MARS_CHECK(a && a->q && a->k && a->v && a->out, "%s: null pointer", what);
     MARS_CHECK(a->dtype == 0 || a->dtype == 1, "%s: dtype %d", what, a->dtype);
     const int es = a->dtype == 1 ? 2 : 4;
-    MARS_CHECK(a->B > 0 && a->Lq > 0 && a->Lk > 0 && a->H > 0 && a->Hkv > 0, "%s: bad shape B=%d Lq=%d Lk=%d H=%d Hkv=%d", what, a->B, a->Lq, a->Lk,
-               a->H, a->Hkv);
-    MARS_CHECK(a->H % a->Hkv == 0, "%s: %d query heads are no multiple of %d key heads", what, a->H, a->Hkv);
-    MARS_CHECK(a->hd > 0 && a->hd <= 128 && (a->hd * es) % 16 == 0, "%s: head dim %d (up to 128, a multiple of 16 bytes)", what, a->hd);
-    MARS_CHECK((int64_t)(a->H / a->Hkv) * a->Lq < (1ll << 30) && a->Lk < (1 << 30), "%s: too many rows", what);
-    MARS_CHECK((int64_t)a->B * a->H < (1ll << 30), "%s: too many heads", what);
+    if (const int rc = check_shape(a, what)) return rc;
+    MARS_CHECK((a->hd * es) % 16 == 0, "%s: head dim %d (up to 128, a multiple of 16 bytes)", what, a->hd);
     MARS_CHECK(a->bias == nullptr || (a->bias_s[1] >= 0 && a->bias_s[1] < (1 << 28)), "%s: bias rows too far apart", what);
     MARS_CHECK(a->scale > 0.f && a->scale < INFINITY, "%s: scale must be positive and finite", what);
     MARS_CHECK(rows_ok(a->q, a->q_s, es) && rows_ok(a->k, a->k_s, es) && rows_ok(a->v, a->v_s, es) && rows_ok(a->out, a->out_s, es),
@@ -542,7 +549,7 @@ int64_t bwd_ws_bytes(const MarsCrossAttn* a);
 }  // namespace xattn
 
 extern "C" int64_t marship_cross_attn_ws(const MarsCrossAttn* a, int backward) {
-    if (a == nullptr || a->B <= 0 || a->Lq <= 0 || a->Lk <= 0 || a->H <= 0 || a->Hkv <= 0 || a->hd <= 0) return 0;
+    if (a == nullptr || xattn::check_shape(a, "cross_attn_ws") != 0) return 0;
     const int64_t keys = xattn::key_ws_bytes(a);
     if (backward) return keys + xattn::bwd_ws_bytes(a);
     return keys + xattn::align256(xattn::plan_fwd(a).part_bytes);
