@@ -241,18 +241,24 @@ __global__ __launch_bounds__(256) void bucket_bias_grad_join_kernel(const float*
     if (wave == 0 && ix < a.nx) dtable[((int64_t)iy * a.nx + ix) * a.H + h] = (acc[0][lane] + acc[1][lane]) + (acc[2][lane] + acc[3][lane]);
 }
 
-int bias_check(const char* what, const void* p, const int32_t* by, const int32_t* bx, const void* t, int H, int qh, int qw, int kh, int kw, int ny, int nx,
-               int64_t sh, int64_t sl) {
-    MARS_CHECK(p && by && bx && t, "%s: null pointer", what);
+// what the workspace query asks too: beyond these the counts of workgroups leave their types; it answers 0 for a shape that the call refuses
+int shape_check(const char* what, int H, int qh, int qw, int kh, int kw, int ny, int nx) {
     MARS_CHECK(H > 0 && qh > 0 && qw > 0 && kh > 0 && kw > 0 && ny > 0 && nx > 0, "%s: empty shape", what);
     MARS_CHECK((int64_t)qh * qw < (1ll << 29) && (int64_t)kh * kw < (1ll << 29) && (int64_t)ny * nx < (1ll << 30), "%s: too many tokens or buckets", what);
     MARS_CHECK(H <= 65535, "%s: %d heads", what, H);
+    return 0;
+}
+
+int bias_check(const char* what, const void* p, const int32_t* by, const int32_t* bx, const void* t, int H, int qh, int qw, int kh, int kw, int ny, int nx,
+               int64_t sh, int64_t sl) {
+    MARS_CHECK(p && by && bx && t, "%s: null pointer", what);
+    if (const int rc = shape_check(what, H, qh, qw, kh, kw, ny, nx)) return rc;
     MARS_CHECK(sl >= (int64_t)kh * kw && (H == 1 || sh >= (int64_t)(qh * qw - 1) * sl + (int64_t)kh * kw), "%s: rows overlap", what);
     return 0;
 }
 
 // the gradient's first launch cut into workgroups: `parts` of them for one head (grid form), or for one head and grid-row offset
-struct GradCut { bool rows; int ndx, ncq, qyn, qxn, nky, parts; };
+struct GradCut { bool rows; int ndx, ncq, qyn, qxn, nky; int64_t parts; };
 GradCut grad_cut(int H, int qh, int qw, int kh, int kw) {
     GradCut c{};
     c.rows = kh >= 8;
@@ -264,13 +270,13 @@ GradCut grad_cut(int H, int qh, int qw, int kh, int kw) {
         if (c.ncq > (qw + 7) / 8) c.ncq = (qw + 7) / 8;
         c.qxn = (qw + c.ncq - 1) / c.ncq;
         c.ncq = (qw + c.qxn - 1) / c.qxn;
-        c.parts = qh * c.ncq * c.nky * c.ndx;
+        c.parts = (int64_t)qh * c.ncq * c.nky * c.ndx;
         return c;
     }
     c.ndx = (qw + kw - 1 + DXC - 1) / DXC;
     c.ncq = (qw + ROWC - 1) / ROWC;
     c.qyn = qw >= ROWC ? 1 : ROWC / qw;
-    c.parts = ((qh + c.qyn - 1) / c.qyn) * c.ncq * c.ndx;
+    c.parts = (int64_t)((qh + c.qyn - 1) / c.qyn) * c.ncq * c.ndx;
     return c;
 }
 
@@ -293,7 +299,7 @@ extern "C" int marship_bucket_bias(const float* table, const int32_t* by, const 
 }
 
 extern "C" int64_t marship_bucket_bias_bwd_ws(int H, int qh, int qw, int kh, int kw, int ny, int nx) {
-    if (H <= 0 || qh <= 0 || qw <= 0 || kh <= 0 || kw <= 0 || ny <= 0 || nx <= 0) return 0;
+    if (shape_check("bucket_bias_bwd_ws", H, qh, qw, kh, kw, ny, nx) != 0) return 0;
     const GradCut c = grad_cut(H, qh, qw, kh, kw);
     return (int64_t)H * c.parts * (c.rows ? (int64_t)ny * nx : (int64_t)(qh + kh - 1) * nx) * 4;
 }
@@ -307,7 +313,7 @@ extern "C" int marship_bucket_bias_bwd(const float* dbias, int64_t s_head, int64
     const BiasArgs a{by, bx, H, qh, qw, kh, kw, ny, nx, s_head, s_row};
     const GradCut c = grad_cut(H, qh, qw, kh, kw);
     if (c.rows) {
-        MARS_CHECK((int64_t)c.parts * 512 < (1ll << 32), "bucket_bias_bwd: more workgroups than a launch takes");
+        MARS_CHECK(c.parts * 512 < (1ll << 32), "bucket_bias_bwd: more workgroups than a launch takes");
         const dim3 grid((unsigned)c.parts, (unsigned)H);
 #define MARS_GRAD_ROWS(KJ)                                                                                                                                  \
     case KJ: hipLaunchKernelGGL((bucket_bias_grad_rows_kernel<KJ>), grid, dim3(512), 0, (hipStream_t)stream, dbias, a, (float*)ws, c.ncq, c.qxn, c.nky, c.ndx); break
@@ -319,17 +325,17 @@ extern "C" int marship_bucket_bias_bwd(const float* dbias, int64_t s_head, int64
 #undef MARS_GRAD_ROWS
         MARS_LAUNCH_CHECK();
         hipLaunchKernelGGL(bucket_bias_grad_rows_join_kernel, dim3((unsigned)((ny * nx + 63) / 64), (unsigned)H), dim3(256), 0, (hipStream_t)stream,
-                           (const float*)ws, a, dtable, c.parts);
+                           (const float*)ws, a, dtable, (int)c.parts);
         MARS_LAUNCH_CHECK();
         return 0;
     }
-    MARS_CHECK(qh + kh - 1 <= 65535 && ny <= 65535 && (int64_t)c.parts * 512 < (1ll << 32), "bucket_bias_bwd: more workgroups than a launch takes");
+    MARS_CHECK(qh + kh - 1 <= 65535 && ny <= 65535 && c.parts * 512 < (1ll << 32), "bucket_bias_bwd: more workgroups than a launch takes");
     hipStream_t s = (hipStream_t)stream;
     hipLaunchKernelGGL(bucket_bias_grad_kernel, dim3((unsigned)c.parts, (unsigned)(qh + kh - 1), (unsigned)H), dim3(512), 0, s, dbias, a, (float*)ws, c.ndx, c.ncq,
                        c.qyn);
     MARS_LAUNCH_CHECK();
     hipLaunchKernelGGL(bucket_bias_grad_join_kernel, dim3((unsigned)((nx + 63) / 64), (unsigned)ny, (unsigned)H), dim3(256), 0, s, (const float*)ws, a, dtable,
-                       c.parts);
+                       (int)c.parts);
     MARS_LAUNCH_CHECK();
     return 0;
 }

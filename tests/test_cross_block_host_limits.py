@@ -14,3 +14,22 @@ def test_workspace_of_a_refused_shape_is_none(pkg, over, backward):
     a = _args(pkg, **over)
     assert lib.marship_cross_attn_ws(ctypes.byref(a), backward) == 0
     assert lib.marship_cross_attn(ctypes.byref(a), None) == -1
+
+
+@pytest.mark.parametrize("shape", [(1 << 30, 1 << 30, 1, 1 << 29, 1, 8, 8), (1, 1 << 15, 1 << 14, 8, 8, 8, 8), (70000, 1, 8, 8, 8, 8, 8), (1, 1, 8, 1 << 29, 1, 8, 8), (0, 1, 8, 1, 8, 1, 8)])
+def test_bias_workspace_of_a_refused_shape_is_none(pkg, shape):
+    """the count of workgroups left 64 bits, came out as zero and was divided by"""
+    lib = pkg.hip.lib()
+    P = ctypes.c_void_p(4096)
+    assert lib.marship_bucket_bias_bwd_ws(*shape) == 0
+    assert lib.marship_bucket_bias_bwd(P, 1 << 62, 1 << 40, P, P, P, *shape, P, 1 << 60, None) == -1
+
+
+def test_bias_workspace_is_counted_in_64_bits(pkg):
+    """2^31 workgroups: the largest grids the call takes, in more than 32 bits (and more than a launch takes)"""
+    lib = pkg.hip.lib()
+    P = ctypes.c_void_p(4096)
+    shape = (1, 1 << 20, 1, 1 << 17, 1, 8, 8)
+    assert lib.marship_bucket_bias_bwd_ws(*shape) == (1 << 31) * 64 * 4
+    assert lib.marship_bucket_bias_bwd(P, 1 << 62, 1 << 17, P, P, P, *shape, P, 1 << 60, None) == -1
+    assert "more workgroups" in lib.marship_last_error().decode()
