@@ -443,7 +443,6 @@ FwdPlan plan_fwd(const MarsCrossAttn* a) {
 template <typename T, int HD> int launch_fwd(const Fwd& f, bool few, hipStream_t s) {
     constexpr int HDP = padded(HD);
     const int64_t blocks = (int64_t)f.p.B * f.p.Hkv * f.nrb * f.ns;
-    MARS_CHECK(blocks * 256 < (1ll << 32), "cross_attn: %lld workgroups are more than a launch takes", (long long)blocks);
     const dim3 grid((unsigned)blocks), block(256);
     if (f.p.bias != nullptr) {
         if (few) hipLaunchKernelGGL((cross_fwd_kernel<T, HD, true, true>), grid, block, 0, s, f);
@@ -457,7 +456,6 @@ template <typename T, int HD> int launch_fwd(const Fwd& f, bool few, hipStream_t
         const int64_t rows = (int64_t)f.p.B * f.p.Hkv * f.p.R;
         const bool deep = f.ns > 4;
         const int64_t per = deep ? 4 : 4 * (64 / (HDP / 4 == 24 ? 32 : HDP / 4)), groups = (rows + per - 1) / per;
-        MARS_CHECK(groups * 256 < (1ll << 32), "cross_attn: more workgroups than a launch takes");
         if (deep) hipLaunchKernelGGL((cross_join_kernel<T, HDP, true>), dim3((unsigned)groups), block, 0, s, f);
         else hipLaunchKernelGGL((cross_join_kernel<T, HDP, false>), dim3((unsigned)groups), block, 0, s, f);
         MARS_LAUNCH_CHECK();
@@ -513,6 +511,12 @@ int check(const MarsCrossAttn* a, bool backward) {
                    "%s: rows must be 16-byte aligned", what);
         MARS_CHECK(a->dbias == nullptr || a->bias != nullptr, "%s: a gradient of a bias that is not there", what);
     }
+    // What the launches take, all of it before the first one: a refused call has written nothing.  (Only launches of fewer than 1024 blocks are cut further.)
+    const int64_t nbh = (int64_t)a->B * a->Hkv, R = (int64_t)(a->H / a->Hkv) * a->Lq, most = 1ll << 24;
+    MARS_CHECK(nbh * ((R + 127) / 128) < most && (!backward || nbh * (((int64_t)a->Lk + 127) / 128) < most), "%s: more workgroups than a launch takes", what);
+    MARS_CHECK(a->mask == nullptr || (int64_t)a->B * 1024 < (1ll << 32), "%s: %d batch entries are more than a launch takes", what, a->B);
+    MARS_CHECK(!backward || a->dbias == nullptr || (((int64_t)a->Lq + 127) / 128 <= 65535 && a->H <= 65535 && ((int64_t)a->Lk + 63) / 64 < most),
+               "%s: more workgroups than a launch takes", what);
     return 0;
 }
 
@@ -535,7 +539,6 @@ int64_t key_ws_bytes(const MarsCrossAttn* a) { return a->mask ? align256((int64_
 
 int prepare_keys(const MarsCrossAttn* a, Prob& p, int32_t* ws, hipStream_t s) {
     if (a->mask == nullptr) return 0;
-    MARS_CHECK((int64_t)a->B * 1024 < (1ll << 32), "cross_attn: %d batch entries are more than a launch takes", a->B);
     int32_t* cnt = (int32_t*)((char*)ws + align256((int64_t)a->B * a->Lk * 4));
     hipLaunchKernelGGL(list_keys_kernel, dim3((unsigned)a->B), dim3(1024), 0, s, a->mask, a->kv_len, a->Lk, ws, cnt);
     MARS_LAUNCH_CHECK();
