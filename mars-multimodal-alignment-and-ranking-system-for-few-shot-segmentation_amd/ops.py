@@ -1103,7 +1103,7 @@ def _cross_block(what, q, k, v, out, stat, scale, kv_len, mask, bias) -> MarsCro
     if bias is not None:
         _req(bias.dtype == torch.float32 and tuple(bias.shape) == (H, Lq, Lk) and (bias.stride(2) == 1 or Lk == 1), f"{what}: bias must be f32 [H, Lq, Lk]")
         a.bias_s = _strides2(bias)
-    scale = hd ** -0.5 if scale is None else float(scale)
+    scale = hd ** -0.5 if scale is None else scale
     _req(0.0 < scale < float("inf"), f"{what}: scale must be positive and finite")
     a.q_s, a.k_s, a.v_s, a.out_s = _strides3(q), _strides3(k), _strides3(v), _strides3(out)
     a.B, a.Lq, a.Lk, a.H, a.Hkv, a.hd, a.scale, a.dtype = B, Lq, Lk, H, Hkv, hd, scale, dt(q)
@@ -1125,6 +1125,7 @@ def cross_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Ten
     without a key gives zeros.  ``scale`` defaults to hd ** -0.5.  ``stat`` f32 [B, H, Lq, 2] receives what ``cross_attn_bwd`` needs."""
     _on_device(q, k, v, out, stat, kv_len, mask, bias)
     lib = hip.lib()
+    scale = None if scale is None else float(scale)             # (a tensor would be known again by its identity)
 
     def build():
         a = _cross_block("cross_attn", q, k, v, out, stat, scale, kv_len, mask, bias)
@@ -1152,6 +1153,7 @@ def cross_attn_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch
     ``bias`` as in the forward call.  Sums have a fixed order: the same call gives the same bits."""
     _on_device(q, k, v, out, stat, dout, dq, dk, dv, dbias, kv_len, mask, bias)
     lib = hip.lib()
+    scale = None if scale is None else float(scale)
 
     def build():
         _req(stat is not None, "cross_attn_bwd: stat of the forward call is needed")

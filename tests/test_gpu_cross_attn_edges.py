@@ -60,3 +60,19 @@ def test_masked_keys_and_absent_keys_give_the_same_gradient(pkg, cuda, how, bias
             bound += float((2 * (n + 8) * U32 * M * 2.0 ** -7 * want[:, h].abs()).sum())
         diff = float((got[b].double() - want).square().sum())
         assert diff <= 4 * bound, f"{n} keys: {(diff / float(want.square().sum())) ** 0.5:.2e} of the norm, bound {(4 * bound / float(want.square().sum())) ** 0.5:.2e}"
+
+
+def test_scale_is_taken_by_value(pkg, cuda):
+    """a scale that comes as a zero-dimensional tensor or a numpy number counts by its value at the call, also the second time"""
+    c = make(cuda, torch.float32, 1, 9, 30, 2, 2, 16, seed=3)
+    stat, res = torch.empty(1, 2, 9, 2, device=cuda), {}
+    outs = lambda: [torch.empty_like(c[n]) for n in ("q", "q", "k", "v")]
+    held = torch.tensor(0.25)
+    for value in (0.25, 0.75):
+        held.fill_(value)
+        for name, scale in (("float", value), ("tensor", held), ("numpy", held.numpy()[()])):
+            out, dq, dk, dv = res[name] = outs()
+            pkg.ops.cross_attn(c["q"], c["k"], c["v"], out, stat=stat, scale=scale)
+            pkg.ops.cross_attn_bwd(c["q"], c["k"], c["v"], out, stat, c["dout"], dq, dk, dv, scale=scale)
+        for name in ("tensor", "numpy"):
+            assert all(torch.equal(a, b) for a, b in zip(res[name], res["float"])), name
