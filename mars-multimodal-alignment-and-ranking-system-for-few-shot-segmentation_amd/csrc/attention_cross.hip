@@ -111,8 +111,8 @@ __global__ __launch_bounds__(256, (FwdCfg<T, HD, FEW>::WPE)) void cross_fwd_kern
     const int64_t kl = p.sk.l * (int)sizeof(T), vl = p.sv.l * (int)sizeof(T);
 
     // The rows that this thread's fills of a tile take; with a list of attended keys they are looked up a tile ahead, so that no fill
-    // waits for its index.  (Keys behind the last attended one: that one again - their scores are set to -inf, and its row holds
-    // no value that the sums would not see anyway.)
+    // waits for its index.  (Keys behind the last attended one: that one again - their scores are set to -inf and
+    // their values to 0, so that an infinity among the last key's is not multiplied by a probability of 0.)
     constexpr int NW = FEW ? 1 : 4, STEP = FEW ? 4 : 1;
     using FL = typename TL::template Fill<KT, NW>;
     const int fw = FEW ? 0 : wave;
@@ -201,7 +201,15 @@ __global__ __launch_bounds__(256, (FwdCfg<T, HD, FEW>::WPE)) void cross_fwd_kern
                 // that do not agree: below the rounding of the result); their sum is taken before the rounding
                 const frag_t<T> pf = pack_step<T>(s[kb], u);
 #pragma unroll
-                for (int m = 0; m < DM; ++m) o[m] = mma(TL::cols(vt, 32 * kb + 16 * u, m, lane), pf, o[m]);
+                for (int m = 0; m < DM; ++m) {
+                    frag_t<T> vc = TL::cols(vt, 32 * kb + 16 * u, m, lane);
+                    if constexpr (!WHOLE) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if (t * KT + 32 * kb + 16 * u + 8 * (e >> 2) + 4 * hh + (e & 3) >= n) vc[e] = (T)0.f;
+                    }
+                    o[m] = mma(vc, pf, o[m]);
+                }
             }
     };
     // whole tiles in the loops, the ragged one behind them: both forms inside one loop would make the compiler carry the accumulators

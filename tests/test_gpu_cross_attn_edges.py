@@ -1,4 +1,6 @@
 """Attention between two token sets where it once went wrong, or could: very large scores with a bias, a few attended keys of a long axis."""
+import math
+
 import pytest
 import torch
 
@@ -76,3 +78,20 @@ def test_scale_is_taken_by_value(pkg, cuda):
             pkg.ops.cross_attn_bwd(c["q"], c["k"], c["v"], out, stat, c["dout"], dq, dk, dv, scale=scale)
         for name in ("tensor", "numpy"):
             assert all(torch.equal(a, b) for a, b in zip(res[name], res["float"])), name
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("Lq", [5, 150])
+@pytest.mark.parametrize("Lk,keys", [(64, "all"), (65, "all"), (33, "all"), (100, "mask"), (100, "len"), (3000, "mask"), (3001, "all")])
+def test_infinite_value_of_the_last_key(pkg, cuda, dtype, Lq, Lk, keys):
+    """an overflowed value of the last attended key is an infinity in its own column of the result and nothing anywhere else, whether a tile of keys ends
+    with that key or not (what a tile holds behind it is that key again)"""
+    c = make(cuda, dtype, 2, Lq, Lk, 4, 2, 64, seed=Lk, keys=keys)
+    last = int(torch.nonzero(c["att"][0]).max())
+    c["v"][0, last, 1, 7] = 0.0
+    want = run(pkg, c, backward=False)["out"].clone()
+    c["v"][0, last, 1, 7] = math.inf
+    got = run(pkg, c, backward=False)["out"]
+    assert bool((got[0, :, 2:, 7] == math.inf).all())
+    got[0, :, 2:, 7] = want[0, :, 2:, 7]
+    assert torch.equal(got, want)
