@@ -154,10 +154,10 @@ __global__ __launch_bounds__(512) void bucket_bias_grad_rows_kernel(const float*
         float v[U][KJ][2];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int q = min(qx + u, qx1 - 1), past = qx + u < qx1 ? 0 : a.kw;      // (columns behind the last: nothing on the grid)
+            const int q = min(qx + u, qx1 - 1), past = qx + u < qx1 ? 0 : NOWHERE;   // (columns behind the last: the sign bit takes any offset off the grid)
             const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(row + (int64_t)(q - qx0) * a.sl), 0, a.kh * a.kw * 4, 0x00027000);
-            const int o0 = (unsigned)(q + ox0 + past) < (unsigned)a.kw ? (q + ox0) * 4 : NOWHERE;
-            const int o1 = (unsigned)(q + ox1 + past) < (unsigned)a.kw ? (q + ox1) * 4 : NOWHERE;
+            const int o0 = (unsigned)((q + ox0) | past) < (unsigned)a.kw ? (q + ox0) * 4 : NOWHERE;
+            const int o1 = (unsigned)((q + ox1) | past) < (unsigned)a.kw ? (q + ox1) * 4 : NOWHERE;
 #pragma unroll
             for (int j = 0; j < KJ; ++j) {
                 v[u][j][0] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rsrc, o0, at[j], 0));
