@@ -436,8 +436,9 @@ FwdPlan plan_fwd(const MarsCrossAttn* a) {
     } else if (!pl.few && blocks < 1024) {
         // Little more than a round of workgroups: some CUs work on one more than the others.  Cutting the keys evens that out where it gains more than
         // the partial results cost (written and read once at memory speed, and a launch) - 1369 queries over 6845 keys, 32 heads of 64: 352 workgroups on
-        // 256 CUs, two cuts, 138 -> 118 us.
-        const double t1 = 4.0 * a->B * a->H * (double)a->Lq * a->Lk * pl.hd / 5e14, round1 = (double)((blocks + 255) / 256);
+        // 256 CUs, two cuts, 138 -> 118 us in bf16; over 1369 keys in f32 205 -> 174 us (48 heads over 2000:
+        // 407 -> 352).  The rates are about what full rounds reach in each type.
+        const double t1 = 4.0 * a->B * a->H * (double)a->Lq * a->Lk * pl.hd / (a->dtype == 1 ? 5e14 : 1e14), round1 = (double)((blocks + 255) / 256);
         double best = t1;
         for (int ns = 2; ns <= 4 && ns <= (tiles + 7) / 8; ++ns) {
             const double t = t1 * (double)((blocks * ns + 255) / 256) / ns / round1 + 8.0 * ns * a->B * a->Hkv * R * pl.hdp / 4e12 + 5e-6;
