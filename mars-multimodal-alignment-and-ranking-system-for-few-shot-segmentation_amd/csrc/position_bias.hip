@@ -8,7 +8,7 @@
 // kx - qx and adds up their diagonals; the offsets of a bucket are joined in LDS, the workgroups' tables in a second launch.  No
 // atomics: the sums have one order.  Two forms of the first launch: on grids with eight key rows or more a workgroup takes one query row of the
 // grid with a wave for every eighth key row, so that it reads whole rows of the gradient; on lines its waves share the query rows.
-// 16 heads, 37 x 37 grid, forward: 26 us (4.6 TB/s); 8 heads, 64 x 64 grid, backward: 101 us (5.3 TB/s; the form for lines took 166 there).
+// 16 heads, 37 x 37 grid, forward: 26 us (4.6 TB/s; 8 and 16 heads, 64 x 64 grid: 116 and 233 us, with stores past the caches 123 and 242); 8 heads, 64 x 64 grid, backward: 101 us (5.3 TB/s; the form for lines took 166 there).
 #include "common.h"
 #include "../../include/mars_hip.h"
 
@@ -30,7 +30,7 @@ constexpr int KXC = 4096;           // key columns a workgroup takes at most
 
 // grid: x = key tiles (kyt * ncx + cx), y = qy * ncq + cq, z = head
 __global__ __launch_bounds__(256) void bucket_bias_kernel(const float* __restrict__ table, const BiasArgs a, float* __restrict__ out, int qxn,
-                                                          int ncq, int kyn, int ncx, int stream) {
+                                                          int ncq, int kyn, int ncx) {
     __shared__ float e[FWD_LDS];
     const int tid = threadIdx.x, h = blockIdx.z;
     const int qy = blockIdx.y / ncq, qx0 = (blockIdx.y - qy * ncq) * qxn, nq = min(qxn, a.qw - qx0);
@@ -49,8 +49,7 @@ __global__ __launch_bounds__(256) void bucket_bias_kernel(const float* __restric
         const int y = i / nkx, x = i - y * nkx;
         const float* er = e + y * ew + x + nq - 1;
         float* oi = o + (int64_t)y * a.kw + x;
-        if (stream) for (int q = 0; q < nq; ++q) __builtin_nontemporal_store(er[-q], oi + q * a.sl);
-        else for (int q = 0; q < nq; ++q) oi[q * a.sl] = er[-q];
+        for (int q = 0; q < nq; ++q) oi[q * a.sl] = er[-q];
     }
 }
 
@@ -292,8 +291,7 @@ extern "C" int marship_bucket_bias(const float* table, const int32_t* by, const 
     if (kyn > kh) kyn = kh;
     const int64_t gx = (int64_t)((kh + kyn - 1) / kyn) * ncx, gy = (int64_t)qh * ncq;
     MARS_CHECK(gx * 256 < (1ll << 32) && gy <= 65535, "bucket_bias: more workgroups than a launch takes");
-    hipLaunchKernelGGL(bucket_bias_kernel, dim3((unsigned)gx, (unsigned)gy, (unsigned)H), dim3(256), 0, (hipStream_t)stream, table, a, out, qxn, ncq, kyn,
-                       ncx, (int)((int64_t)H * qh * qw * kh * kw >= (1ll << 26)));
+    hipLaunchKernelGGL(bucket_bias_kernel, dim3((unsigned)gx, (unsigned)gy, (unsigned)H), dim3(256), 0, (hipStream_t)stream, table, a, out, qxn, ncq, kyn, ncx);
     MARS_LAUNCH_CHECK();
     return 0;
 }
