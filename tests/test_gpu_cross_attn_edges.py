@@ -1,4 +1,5 @@
 """Attention between two token sets where it once went wrong, or could: very large scores with a bias, a few attended keys of a long axis."""
+import ctypes
 import math
 
 import pytest
@@ -95,3 +96,13 @@ def test_infinite_value_of_the_last_key(pkg, cuda, dtype, Lq, Lk, keys):
     assert bool((got[0, :, 2:, 7] == math.inf).all())
     got[0, :, 2:, 7] = want[0, :, 2:, 7]
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype,Lq,Lk", [(torch.float32, 300, 1100), (torch.bfloat16, 300, 5000)])
+@pytest.mark.parametrize("keys,bias", [("all", None), ("mask", "rand")])
+def test_keys_cut_where_a_round_of_workgroups_is_left_over(pkg, cuda, dtype, Lq, Lk, keys, bias):
+    """384 blocks of query rows on 256 CUs: the keys are cut in two or more and joined"""
+    c = make(cuda, dtype, 2, Lq, Lk, 64, 64, 64, seed=7, keys=keys, bias=bias)
+    a = pkg.ops._cross_block("test", c["q"], c["k"], c["v"], torch.empty_like(c["q"]), None, c["scale"], c["kv_len"], None, c["bias"])
+    assert pkg.hip.lib().marship_cross_attn_ws(ctypes.byref(a), 0) > 0
+    check(pkg, c, backward=False)
