@@ -606,10 +606,14 @@ int vec_width(int Cg, std::initializer_list<uint64_t> addresses, int es) {
 // the group kernels hold raw vectors: 16 bytes of the wider type (f32: 4 channels)
 int vec_for_group(const Norm& a, int dt_a, int dt_b) { return a.V == 8 && (dt_a == 0 || dt_b == 0) ? 4 : a.V; }
 
+// The map is read twice, so stores that would push it out of the last-level cache go past it.  With n maps of 64 x 64 x 256, forward / step, us:
+//   results in bf16   n = 8: 20.0 / 44 past the cache, 19.8 / 48 through it   n = 16: 24.5 / 70, 27.3 / 76   n = 64: 72 / 221, 75 / 235   n = 96: 109 / 378, 126 / 427
+//   results in f32    n = 16: 45 / 111, 39 / 104   n = 32: 80 / 205, 69 / 206   n = 48: 121 / 327, 126 / 368   n = 64: 152 / 437, 170 / 461
+// (an f32 vector of eight channels is two stores of half a line each: they want the cache for as long as it holds them)
+bool past_cache(const Norm& a, int es) { return (int64_t)a.N * a.P * a.C >= (es == 2 ? 1ll << 24 : 3ll << 24); }
+
 // chunks of rows: about 1024 workgroups, at least KR rows a thread
 void cut(Norm& a) {
-    // the map is read twice: stores that would push it out of the last-level cache go past it (128 x 128 x 256 x 16 bf16: 94 -> 78 us)
-    a.stream = (int64_t)a.N * a.P * a.C >= (1 << 24);
     a.vpr = a.C / a.V;
     a.ncb = (a.vpr + TH - 1) / TH;
     const int nrl = TH / (a.vpr < TH ? a.vpr : TH), least = nrl * KR;
@@ -688,6 +692,7 @@ extern "C" int marship_group_norm_act(const void* x, int64_t x_n, int64_t x_p, c
     const int vw = vx < vo ? vx : vo;
     a.V = vw;
     cut(a);
+    a.stream = past_cache(a, oe);
     MARS_CHECK((int64_t)a.chunks < (1 << 23) && a.ncb <= 65535 && (int64_t)N * G < (1 << 22), "group_norm_act: more workgroups than a launch takes");
     hipStream_t s = (hipStream_t)stream;
     a.V = vec_for_group(a, x_dtype, out_dtype);
@@ -739,6 +744,7 @@ extern "C" int marship_group_norm_act_bwd(const void* x, int64_t x_n, int64_t x_
     const int vw = vx < vy ? vx : vy;
     a.V = vw;
     cut(a);
+    a.stream = past_cache(a, xe);
     MARS_CHECK((int64_t)a.chunks < (1 << 23) && a.ncb <= 65535 && (int64_t)N * G < (1 << 22), "group_norm_act_bwd: more workgroups than a launch takes");
     NormBwd d{};
     d.dy = dy; d.dy_n = dy_n; d.dy_p = dy_p; d.dx = dx; d.dx_n = dx_n; d.dx_p = dx_p; d.stat = stat; d.dw = dw; d.db = db;
