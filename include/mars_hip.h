@@ -172,11 +172,14 @@ int marship_flash_attn_mean(const void* qkv, const float* lse, int T, int H, int
 /* softmax(scale q.k + bias) v of Lq query tokens over the attended ones of Lk key tokens (no counterpart in the reference, whose
  * one attention between two sets is the mask decoder's: marship_attn_small).  Everything is a strided view, strides in
  * elements in the order (batch entry, token, head), the elements of a head contiguous, rows 16-byte aligned; hd <= 128,
- * hd elements a multiple of 16 bytes.  dtype (0 f32, 1 bf16) is that of q, k, v, out and their gradients; products, scores, statistics and
- * sums are f32 (f32 operands go through the f32 matrix instructions).
+ * hd elements a multiple of 16 bytes.  dtype (0 f32, 1 bf16) is that of q, k, v, out and their gradients; scores, statistics and
+ * sums are f32.  f32 operands go through the f32 matrix instructions and are rounded nowhere.  With bf16 operands what is multiplied by V, K, Q and dout is
+ * rounded to bf16 too: the exponentials in the forward call, the probabilities and dS in the backward one (but dS of dq in two bf16 terms where an entry attends to
+ * up to 256 keys, and dbias from the f32 dS).
  *   H query heads share Hkv key heads in order: query head h reads key head h / (H / Hkv).
  *   kv_len i32 [B] (may be NULL): keys at or behind it are not attended (clamped to 0 .. Lk).  mask u8 [B, Lk], contiguous (may be NULL): keys
- *   with 0 are not attended.  What K and V hold at keys that are not attended is not read.
+ *   with 0 are not attended.  What K and V hold at keys that are not attended reaches no result (rows behind kv_len, and masked ones but where dbias is asked for, are not
+ *   even read).
  *   bias f32 [H, Lq, Lk] by bias_s = (head, query row), shared by the batch (may be NULL); -inf and the lowest float are allowed.
  * A row without a key (none attended, or a bias of -inf on all of them) gives zeros and stat (-inf, 0).
  * stat f32 [B, H, Lq, 2]: maximum of the row's scores and sum of exp(score - maximum); written by the forward call where not NULL, read by the
@@ -224,7 +227,8 @@ int marship_bucket_bias_bwd(const float* dbias, int64_t s_head, int64_t s_row, c
 /* x [N, P, C] (strides x_n, x_p in elements, channels contiguous), G groups of C / G neighbouring channels:
  * out = act(w (x - mean) rstd + b) with the mean and variance of a group's P C / G values.  No counterpart in the reference (its channels-last
  * norm is LayerNorm2d: marship_layernorm_act_rows).  act: 0 none, 1 erf GELU, 2 QuickGELU, 3 ReLU, 4 SiLU.  x and out f32 or bf16 each; w, b f32 [C].
- * stat f32 [N, G, 2] receives mean and rstd where not NULL; the backward call reads it.
+ * stat f32 [N, G, 2] receives mean and rstd where not NULL; the backward call reads it.  The erf GELU and its slope keep f32's relative precision in the tail (but for the
+ * roundings of z^2 / 2 in the exponent).
  * Backward: dx (x's dtype), dw, db f32 [C]; dy f32 or bf16.  Statistics and sums are f32 in a fixed order.  ws: at least
  * marship_group_norm_act_ws bytes, 16-byte aligned. */
 int64_t marship_group_norm_act_ws(int N, int P, int C, int G, int backward);

@@ -14,8 +14,8 @@
 //
 // Few rows (one new token a sequence) are bound by memory: the four waves of a workgroup take key tiles in turn through buffers of their own, the keys
 // are cut over the chip and joined (16 sequences over up to 8192 keys, 16 / 4 heads of 128: 40 us for 206 MB).  Many rows are bound by
-// vector ALU: a score costs 16 cycles of exponential and 14 of other work against 8 (64-wide heads) of matrix instructions;
-// 1369 over 6845, 32 heads of 64: 116 us with the join of two cuts, 660 TFLOP/s.
+// vector ALU and matrix pipe one after the other: a wave's 64 scores cost 16 cycles of exponential and 14 of other vector work, and 16 (64-wide heads) in the
+// two products; 1369 over 6845, 32 heads of 64: 115 us with the join of two cuts, 668 TFLOP/s.
 #include <type_traits>
 #include "attention_cross.h"
 

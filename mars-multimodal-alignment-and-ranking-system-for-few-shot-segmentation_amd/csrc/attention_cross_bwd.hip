@@ -16,7 +16,8 @@
 // With one attended key P is 1 whatever the score and dS is 0: dQ, dK and dbias are set to it, because dP - D is the difference of two roundings of one number.
 // Recomputing S and dP in each pass costs 2 of 7 products more than one pass over all would, but that one would add into dQ from
 // every key block: atomics, in an order that changes.
-// 8 x 16 heads of 64, 1369 queries over 684 keys on average: queries 90 us, keys 109 (680 and 560 TFLOP/s of their own products); 2 x 16 heads of 80, 4096 x 4096: 410 and 465 us.
+// 8 x 16 heads of 64, 1369 queries over 684 keys on average: queries 87 us, keys 107 (705 and 575 TFLOP/s of their own products); 2 x 16 heads of 80,
+// 4096 x 4096: 376 and 430 us in a kernel trace, 741 as a call without one.
 #include <type_traits>
 #include "attention_cross.h"
 
@@ -463,6 +464,7 @@ __global__ __launch_bounds__(256) void cross_bwd_sum_kernel(const Bwd f) {
 // dbias[h, i, j] = sum_b dS: grid (key tiles of 64, query blocks of 128, heads); keys are taken where they stand (the lists of attended keys
 // differ from entry to entry), with the key as lane column so that rows of bias and dbias are read and written in whole lines.  While one
 // batch entry is worked on, the next one's K and V tiles, query rows and row values are on their way.
+// (A masked key below kv_len is loaded with the others of its tile.  Keys are lane columns: what it holds stays in its own, which is not used.)
 template <typename T, int HD>
 __global__ __launch_bounds__(256, (HD <= 64 && sizeof(T) == 2) ? 2 : 1) void cross_bwd_bias_kernel(const Bwd f) {
     constexpr int HDP = padded(HD);
